@@ -251,7 +251,7 @@ def _own(s):
         return q[:, :K].view(torch.float8_e4m3fn), scale
     if s["op"] == "dense":
         y = torch.empty((s["M"], s["N"]), device="cuda", dtype=DTYPES[s["dtype"]])
-        _call("rg_dense_e4m3", s["xq"].data_ptr(), s["xq"].stride(0), s["xs"].data_ptr(), s["xs"].stride(0), s["wq"].data_ptr(), s["wq"].stride(0), s["ws"].data_ptr(),
+        _call("rg_dense_e4m3", s["xq"].data_ptr(), s["xq"].stride(0), s["xs"].data_ptr(), s["M"], s["wq"].data_ptr(), s["wq"].stride(0), s["ws"].data_ptr(),
               None if s["b"] is None else s["b"].data_ptr(), y.data_ptr(), s["N"], RG_DTYPES[s["dtype"]], s["M"], s["N"], s["K"])
         return y
     q, kv, kvd = s["q"], s["kv"], s["kv_heads"] * s["dim"]
