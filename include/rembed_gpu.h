@@ -261,6 +261,42 @@ int rg_quantize_rows_s8(const void *x, int M, int K, int8_t *q, float *row_scale
 int rg_dense_s8(const int8_t *xq, const float *row_scale, const int8_t *wq, const float *col_scale, const float *bias,
                 float *y, int M, int N, int K, void *stream, char **err);
 
+/* ---- 8-bit floating point with a scale per block of 128 ----------------
+ * No counterpart in the reference.  e4m3 values (1 sign, 4 exponent, 3
+ * mantissa bits, largest 448) with one fp32 scale per block: a block of an
+ * activation is 128 consecutive values of one row, a block of a weight is a
+ * tile of 128 rows x 128 columns; the last block of a row or column may be
+ * shorter.  What a value stands for is e4m3 * scale.
+ *
+ * rg_quantize_rows_e4m3: x [M x K] (row stride ldx elements; RG_DTYPE_F32,
+ * F16 or BF16) -> q [M x K] e4m3 bytes (row stride ldq; columns from K on are
+ * left alone) and scale[b * ld_scale + m] for block b of row m, b <
+ * ceil(K / 128), ld_scale >= M.  scale = maxabs(block) / 448 (1 for a block
+ * of zeros, at least 2^-126), q = e4m3(x * (1 / scale)), to nearest, ties to
+ * even, clamped to +-448.  A block with a NaN or an infinity stands for NaNs.
+ * rg_dense_e4m3 reads q with ldq a multiple of 16 from a 16-byte aligned
+ * base.
+ *
+ * rg_quantize_tiles_e4m3: the same for the tiles of a weight w [N x K]:
+ * scale[(n / 128) * ceil(K / 128) + b], contiguous. */
+int rg_quantize_rows_e4m3(const void *x, int dtype, int ldx, int M, int K, uint8_t *q, int ldq, float *scale,
+                          int ld_scale, void *stream, char **err);
+int rg_quantize_tiles_e4m3(const void *w, int dtype, int ldw, int N, int K, uint8_t *q, int ldq, float *scale,
+                           void *stream, char **err);
+
+/* rg_dense_e4m3: the projection over such operands,
+ * y[m][n] = sum_b x_scale[b * ld_xs + m] * w_scale[n / 128][b] *
+ *           sum_{k in block b} xq[m][k] * wq[n][k]   (+ bias[n]),
+ * every sum in fp32.  xq [M x K] and wq [N x K] e4m3 with row strides ldx,
+ * ldw (multiples of 16, 16-byte aligned bases; columns from K on are not
+ * read), scales as the quantisers write them, bias fp32 or NULL, y [M x N]
+ * with row stride ldy in `dtype` (RG_DTYPE_F32, F16 or BF16; columns from N
+ * on are left alone).  Any M, N, K >= 1 (M up to 8 388 480).  An fp16 result
+ * beyond 65504 raises the overflow status (rg_kernel_status).  Deterministic. */
+int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, const uint8_t *wq, int ldw,
+                  const float *w_scale, const float *bias, void *y, int ldy, int dtype, int M, int N, int K,
+                  void *stream, char **err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 // kernel_abi.cu - kernel-level C ABI entry points beyond the dense
 // projections: varlen attention, the full-int8 row quantiser and integer
-// GEMM, and the status check shared by every kernel-level call.
+// GEMM, the e4m3 quantisers and block-scaled GEMM, and the status check
+// shared by every kernel-level call.
 //
 // These calls take device pointers on the current CUDA device and are
 // asynchronous on the caller's stream.  A failure that a kernel detects on
@@ -21,6 +22,7 @@
 #include <string>
 
 #include "rembed_gpu.h"
+#include "e4m3.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
@@ -85,6 +87,40 @@ cudaError_t kernel_status_word(int dev, int** out) {
 cudaError_t noalloc_status_take(int* s);
 
 }  // namespace rg
+
+namespace {
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// Size of an RG_DTYPE_* element, 0 for an unknown one.
+unsigned dtype_size(int dtype) {
+    return dtype == RG_DTYPE_F32 ? 4 : (dtype == RG_DTYPE_F16 || dtype == RG_DTYPE_BF16 ? 2 : 0);
+}
+
+rg::Elem elem_of(int dtype) {
+    return dtype == RG_DTYPE_F32 ? rg::Elem::kF32 : (dtype == RG_DTYPE_F16 ? rg::Elem::kF16 : rg::Elem::kBF16);
+}
+
+// The two e4m3 quantisers' common checks; fills p.
+int quant_e4m3_args(const char* fn, const void* x, int dtype, int ldx, int rows, int K, uint8_t* q, int ldq,
+                    float* scale, rg::QuantE4Params* p, char** err) {
+    if (!x || !q || !scale) return set_err(err, "%s: null buffer", fn);
+    const unsigned size = dtype_size(dtype);
+    if (!size) return set_err(err, "%s: unknown dtype %d", fn, dtype);
+    if (K <= 0) return set_err(err, "%s: K=%d must be positive", fn, K);
+    if (ldx < K || ldq < K) return set_err(err, "%s: a row stride is narrower than K=%d", fn, K);
+    if (misaligned(x, size) || misaligned(scale, 4)) return set_err(err, "%s: a buffer is not aligned to its type", fn);
+    p->x = x;
+    p->ldx = ldx;
+    p->rows = rows;
+    p->K = K;
+    p->q = q;
+    p->ldq = ldq;
+    p->scale = scale;
+    return 0;
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -222,6 +258,73 @@ int rg_dense_s8(const int8_t* xq, const float* row_scale, const int8_t* wq, cons
     a.status = status;
     e = rg::gemm_launch(rg::GemmKind::kS8, rg::kEpiBiasF32, bn, ta, tb, a, sms, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return set_err(err, "rg_dense_s8: launch: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int rg_quantize_rows_e4m3(const void* x, int dtype, int ldx, int M, int K, uint8_t* q, int ldq, float* scale,
+                          int ld_scale, void* stream, char** err) {
+    if (M <= 0) return 0;
+    rg::QuantE4Params p{};
+    if (quant_e4m3_args("rg_quantize_rows_e4m3", x, dtype, ldx, M, K, q, ldq, scale, &p, err) != 0) return -1;
+    if (ld_scale < M) return set_err(err, "rg_quantize_rows_e4m3: ld_scale=%d is below M=%d", ld_scale, M);
+    p.ld_scale = ld_scale;
+    cudaError_t e = rg::launch_quantize_rows_e4m3(elem_of(dtype), p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return set_err(err, "rg_quantize_rows_e4m3: launch: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int rg_quantize_tiles_e4m3(const void* w, int dtype, int ldw, int N, int K, uint8_t* q, int ldq, float* scale,
+                           void* stream, char** err) {
+    if (N <= 0) return 0;
+    rg::QuantE4Params p{};
+    if (quant_e4m3_args("rg_quantize_tiles_e4m3", w, dtype, ldw, N, K, q, ldq, scale, &p, err) != 0) return -1;
+    if (N > 65535 * rg::kE4Block) return set_err(err, "rg_quantize_tiles_e4m3: N=%d is over %d", N, 65535 * rg::kE4Block);
+    cudaError_t e = rg::launch_quantize_tiles_e4m3(elem_of(dtype), p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return set_err(err, "rg_quantize_tiles_e4m3: launch: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int rg_dense_e4m3(const uint8_t* xq, int ldx, const float* x_scale, int ld_xs, const uint8_t* wq, int ldw,
+                  const float* w_scale, const float* bias, void* y, int ldy, int dtype, int M, int N, int K,
+                  void* stream, char** err) {
+    if (M <= 0) return 0;
+    if (!xq || !x_scale || !wq || !w_scale || !y) return set_err(err, "rg_dense_e4m3: null buffer");
+    const unsigned size = dtype_size(dtype);
+    if (!size) return set_err(err, "rg_dense_e4m3: unknown dtype %d", dtype);
+    if (N <= 0 || K <= 0) return set_err(err, "rg_dense_e4m3: N=%d and K=%d must be positive", N, K);
+    if (ldx < K || ldw < K || ldy < N || ld_xs < M)
+        return set_err(err, "rg_dense_e4m3: a row stride is narrower than its row (K=%d N=%d M=%d)", K, N, M);
+    if (ldx % 16 != 0 || ldw % 16 != 0 || misaligned(xq, 16) || misaligned(wq, 16))
+        return set_err(err, "rg_dense_e4m3: e4m3 rows must start on 16-byte boundaries (ldx=%d ldw=%d)", ldx, ldw);
+    if (misaligned(x_scale, 4) || misaligned(w_scale, 4) || misaligned(bias, 4) || misaligned(y, size))
+        return set_err(err, "rg_dense_e4m3: a buffer is not aligned to its type");
+    if (M > 65535 * 128) return set_err(err, "rg_dense_e4m3: M=%d is over %d", M, 65535 * 128);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return set_err(err, "cudaGetDevice: %s", cudaGetErrorString(e));
+    int sms = 148;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return set_err(err, "cudaDeviceGetAttribute: %s", cudaGetErrorString(e));
+    int* status = nullptr;
+    e = rg::kernel_status_word(dev, &status);
+    if (e != cudaSuccess) return set_err(err, "rg_dense_e4m3: status word: %s", cudaGetErrorString(e));
+    rg::DenseE4Params p{};
+    p.xq = xq;
+    p.wq = wq;
+    p.ldx = ldx;
+    p.ldw = ldw;
+    p.x_scale = x_scale;
+    p.ld_xs = ld_xs;
+    p.w_scale = w_scale;
+    p.bias = bias;
+    p.y = y;
+    p.ldy = ldy;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.status = status;
+    e = rg::launch_dense_e4m3(elem_of(dtype), p, sms, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return set_err(err, "rg_dense_e4m3: launch: %s", cudaGetErrorString(e));
     return 0;
 }
 

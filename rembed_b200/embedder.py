@@ -125,6 +125,13 @@ SIGNATURES = {
     "rg_quantize_rows_s8": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.c_int, _VP, _VP, _VP, _ERR]),
     "rg_dense_s8": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
                                    _ERR]),
+    "rg_quantize_rows_e4m3": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
+                                             ctypes.c_int, _VP, ctypes.c_int, _VP, _ERR]),
+    "rg_quantize_tiles_e4m3": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
+                                              ctypes.c_int, _VP, _VP, _ERR]),
+    "rg_dense_e4m3": (ctypes.c_int, [_VP, ctypes.c_int, _VP, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP, _VP,
+                                     ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
+                                     _ERR]),
 }
 
 _lib = None
