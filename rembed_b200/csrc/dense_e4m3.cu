@@ -31,39 +31,43 @@ __device__ __forceinline__ void store_y(void* y, int64_t at, float v) {
 }
 
 // ---------------------------------------------------------------------------
-// Weight rows on the M side of the MMA: a CTA owns 128 weight rows (one
-// weight block, so its weight scale is one number per block of K) and NT rows
-// of x.  Roles (256 threads):
+// Few rows of x: weight rows on the M side of the MMA.  A CTA owns 128 weight
+// rows (one weight block, so its weight scale is one number per block of K)
+// and NT rows of x, over its share of K; the shares of a cluster's CTAs are
+// joined through distributed shared memory, in rank order.  Such products
+// wait for the weights: at M <= 64 the CTAs of a wave keep two times four
+// stages of 16 KB of them in flight per SM.  Roles (256 threads):
 //   warp 0     TMA producer: 128 weight rows and NT x rows of each k-block;
-//   warp 1     MMA issuer (one thread), four MMAs per k-block into one of ACC
-//              accumulators;
-//   warp 2     TMEM allocator, then the scales: xs * ws of each k-block into
-//              a ring in shared memory;
-//   warps 4-7  accumulation, thread = weight row = TMEM lane, NT sums each;
-//              the stores of a warp are 32 neighbouring columns of y.
+//   warp 1     MMA issuer, four MMAs per k-block into one of ACC accumulators;
+//   warp 2     TMEM allocator, then the scales of each k-block into a ring in
+//              shared memory (asynchronous copies: loads into registers, one
+//              k-block at a time, held everything else up);
+//   warps 4-7  accumulation, thread = weight row = TMEM lane, NT sums each.
 template <int NT>
 struct ThinShape {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = NT * 128;
-    static constexpr int STAGES = NT == 128 ? 6 : 8;
-    static constexpr int ACC = NT == 128 ? 2 : 4;
-    static constexpr uint32_t TMEM_COLS = ACC * NT < 32 ? 32 : ACC * NT;
-    static constexpr int SR = 8;  // ring of scales
-    static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + SR * NT * 4 + 1024 + 512;
+    static constexpr int STAGES = NT == 128 ? 6 : 4;
+    static constexpr int ACC = 4;
+    static constexpr uint32_t TMEM_COLS = ACC * NT;
+    static constexpr int SR = 8;           // ring of scales
+    static constexpr int SLOT = NT + 4;    // x scales, then the weight scale
+    static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + SR * SLOT * 4 + 1024 + 512;
     static constexpr int THREADS = 256;
+    static_assert(STAGES * (A_BYTES + B_BYTES) >= NT * 512, "the sums of a CTA take the place of its stages");
 };
 
 template <int NT, Elem O>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(256, NT == 128 ? 1 : 2)
     dense_e4m3_thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                           DenseE4Params p) {
+                           DenseE4Params p, int split) {
     using S = ThinShape<NT>;
     constexpr int STAGES = S::STAGES, ACC = S::ACC, SR = S::SR;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sA = smem;
     uint8_t* sB = sA + STAGES * S::A_BYTES;
-    float* sScale = reinterpret_cast<float*>(sB + STAGES * S::B_BYTES);  // [SR][NT]
-    uint64_t* full = reinterpret_cast<uint64_t*>(sScale + SR * NT);
+    float* sScale = reinterpret_cast<float*>(sB + STAGES * S::B_BYTES);  // [SR][SLOT]
+    uint64_t* full = reinterpret_cast<uint64_t*>(sScale + SR * S::SLOT);
     uint64_t* empty = full + STAGES;
     uint64_t* tfull = empty + STAGES;
     uint64_t* tempty = tfull + ACC;
@@ -73,9 +77,12 @@ __global__ void __launch_bounds__(256, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int kblocks = (p.K + kE4Block - 1) / kE4Block;
-    const int nb = blockIdx.x, n0 = nb * 128, m0 = blockIdx.y * NT;
+    const int rank = blockIdx.x % split;  // its share of K: blocks [k0, k0 + nk)
+    const int k0 = static_cast<int>(static_cast<int64_t>(kblocks) * rank / split);
+    const int nk = static_cast<int>(static_cast<int64_t>(kblocks) * (rank + 1) / split) - k0;
+    const int nb = blockIdx.x / split, n0 = nb * 128, m0 = blockIdx.y * NT;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -87,7 +94,7 @@ __global__ void __launch_bounds__(256, 1)
             mbar_init(&tempty[a], 4);
         }
         for (int s = 0; s < SR; ++s) {
-            mbar_init(&cfull[s], 1);
+            mbar_init(&cfull[s], 32);  // the copies of every lane of the scale warp
             mbar_init(&cempty[s], 4);
         }
         mbar_init(drain, 1);
@@ -107,79 +114,80 @@ __global__ void __launch_bounds__(256, 1)
     pdl_wait();
     const uint32_t tmem = *tmem_slot;
 
+    float sum[NT];
     if (warp == 0) {
-        if (lane == 0) {
-            int issued = 0;
-            for (int kb = 0; kb < kblocks; ++kb) {
-                const int s = kb % STAGES;
-                if (!mbar_wait(&empty[s], ((kb / STAGES) & 1) ^ 1, p.status, abort_flag)) break;
+        int issued = 0;
+        for (int kb = 0; kb < nk; ++kb) {
+            const int s = kb % STAGES;
+            if (!mbar_wait_warp(&empty[s], ((kb / STAGES) & 1) ^ 1, p.status, abort_flag)) break;
+            if (elect_one()) {
                 mbar_arrive_expect_tx(&full[s], S::A_BYTES + S::B_BYTES);
-                tma_load_2d(sA + s * S::A_BYTES, &tmW, &full[s], kb * 128, n0);
-                tma_load_2d(sB + s * S::B_BYTES, &tmX, &full[s], kb * 128, m0);
-                issued = kb + 1;
+                tma_load_2d(sA + s * S::A_BYTES, &tmW, &full[s], (k0 + kb) * 128, n0);
+                tma_load_2d(sB + s * S::B_BYTES, &tmX, &full[s], (k0 + kb) * 128, m0);
             }
-            // every load issued has landed before the CTA may exit
-            for (int kb = issued > STAGES ? issued - STAGES : 0; kb < issued; ++kb)
-                mbar_drain(&full[kb % STAGES], (kb / STAGES) & 1);
+            __syncwarp();
+            issued = kb + 1;
         }
+        // every load issued has landed before the CTA may exit
+        for (int kb = issued > STAGES ? issued - STAGES : 0; kb < issued; ++kb)
+            mbar_drain(&full[kb % STAGES], (kb / STAGES) & 1);
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(128, NT);
-            bool issued = false;
-            for (int kb = 0; kb < kblocks; ++kb) {
-                const int s = kb % STAGES, a = kb % ACC;
-                if (!mbar_wait(&tempty[a], ((kb / ACC) & 1) ^ 1, p.status, abort_flag) ||
-                    !mbar_wait(&full[s], (kb / STAGES) & 1, p.status, abort_flag))
-                    break;
-                tc_fence_after();
-                const uint64_t ad = sdesc_k128(smem_u32(sA + s * S::A_BYTES));
-                const uint64_t bd = sdesc_k128(smem_u32(sB + s * S::B_BYTES));
+        constexpr uint32_t idesc = idesc_e4m3(128, NT);
+        const uint64_t ad0 = sdesc_k128(smem_u32(sA)), bd0 = sdesc_k128(smem_u32(sB));
+        bool issued = false;
+        for (int kb = 0; kb < nk; ++kb) {
+            const int s = kb % STAGES, a = kb % ACC;
+            if (!mbar_wait_warp(&tempty[a], ((kb / ACC) & 1) ^ 1, p.status, abort_flag) ||
+                !mbar_wait_warp(&full[s], (kb / STAGES) & 1, p.status, abort_flag))
+                break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t ad = ad0 + s * (S::A_BYTES / 16), bd = bd0 + s * (S::B_BYTES / 16);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) umma_f8(tmem + a * NT, ad + 2 * k, bd + 2 * k, idesc, k > 0);
-                issued = true;
                 umma_commit(&empty[s]);
                 umma_commit(&tfull[a]);
             }
-            if (issued) {
-                umma_commit(drain);
-                mbar_drain(drain, 0);
-            }
+            __syncwarp();
+            issued = true;
+        }
+        if (issued) {
+            if (elect_one()) umma_commit(drain);
+            mbar_drain(drain, 0);
         }
     } else if (warp == 2) {
-        const float* ws = p.w_scale + static_cast<int64_t>(nb) * kblocks;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        const float* xs = p.x_scale + k0 * p.ld_xs + m0 + lane;
+        const float* ws = p.w_scale + static_cast<int64_t>(nb) * kblocks + k0;
+        for (int kb = 0; kb < nk; ++kb) {
             const int c = kb % SR;
-            const float w = __ldg(ws + kb);
-            float v[(NT + 31) / 32];
+            if (!mbar_wait_warp(&cempty[c], ((kb / SR) & 1) ^ 1, p.status, abort_flag)) break;
+            float* to = sScale + c * S::SLOT;
 #pragma unroll
-            for (int i = 0; i < (NT + 31) / 32; ++i) {
-                const int m = m0 + lane + 32 * i;
-                v[i] = m < p.M && lane + 32 * i < NT ? __ldg(p.x_scale + kb * p.ld_xs + m) * w : 0.f;
-            }
-            if (!mbar_wait(&cempty[c], ((kb / SR) & 1) ^ 1, p.status, abort_flag)) break;
-#pragma unroll
-            for (int i = 0; i < (NT + 31) / 32; ++i)
-                if (lane + 32 * i < NT) sScale[c * NT + lane + 32 * i] = v[i];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&cfull[c]);
+            for (int i = 0; i < NT; i += 32)
+                if (lane + i < NT) {  // rows past the end: zeros
+                    const bool in = m0 + lane + i < p.M;
+                    cp_async_f32(to + lane + i, in ? xs + i : p.x_scale, in);
+                }
+            if (lane == 0) cp_async_f32(to + NT, ws + kb, true);
+            cp_async_arrive(&cfull[c]);
+            xs += p.ld_xs;
         }
+        cp_async_wait_all();
     } else if (warp >= 4) {
-        const int quarter = warp & 3;
-        const int n = n0 + quarter * 32 + lane;
-        const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-        float acc[NT];
+        const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i] = 0.f;
+        for (int i = 0; i < NT; ++i) sum[i] = 0.f;
         bool ok = true;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        for (int kb = 0; kb < nk; ++kb) {
             const int a = kb % ACC, c = kb % SR;
-            if (!mbar_wait(&cfull[c], (kb / SR) & 1, p.status, abort_flag) ||
-                !mbar_wait(&tfull[a], (kb / ACC) & 1, p.status, abort_flag)) {
+            if (!mbar_wait_warp(&cfull[c], (kb / SR) & 1, p.status, abort_flag) ||
+                !mbar_wait_warp(&tfull[a], (kb / ACC) & 1, p.status, abort_flag)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const float4* sc = reinterpret_cast<const float4*>(sScale + c * NT);
+            const float4* sc = reinterpret_cast<const float4*>(sScale + c * S::SLOT);
+            const float w = sScale[c * S::SLOT + NT];
 #pragma unroll
             for (int h = 0; h < NT / 16; ++h) {
                 uint32_t t[16];
@@ -188,10 +196,11 @@ __global__ void __launch_bounds__(256, 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float4 s4 = sc[h * 4 + i];
-                    acc[h * 16 + 4 * i + 0] = fmaf(__uint_as_float(t[4 * i + 0]), s4.x, acc[h * 16 + 4 * i + 0]);
-                    acc[h * 16 + 4 * i + 1] = fmaf(__uint_as_float(t[4 * i + 1]), s4.y, acc[h * 16 + 4 * i + 1]);
-                    acc[h * 16 + 4 * i + 2] = fmaf(__uint_as_float(t[4 * i + 2]), s4.z, acc[h * 16 + 4 * i + 2]);
-                    acc[h * 16 + 4 * i + 3] = fmaf(__uint_as_float(t[4 * i + 3]), s4.w, acc[h * 16 + 4 * i + 3]);
+                    float* to = sum + h * 16 + 4 * i;
+                    to[0] = fmaf(__uint_as_float(t[4 * i + 0]), s4.x * w, to[0]);
+                    to[1] = fmaf(__uint_as_float(t[4 * i + 1]), s4.y * w, to[1]);
+                    to[2] = fmaf(__uint_as_float(t[4 * i + 2]), s4.z * w, to[2]);
+                    to[3] = fmaf(__uint_as_float(t[4 * i + 3]), s4.w * w, to[3]);
                 }
             }
             tc_fence_before();
@@ -201,26 +210,389 @@ __global__ void __launch_bounds__(256, 1)
                 mbar_arrive(&cempty[c]);
             }
         }
-        if (ok && n < p.N) {
-            const float b = p.bias ? __ldg(p.bias + n) : 0.f;
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int m = m0 + i;
-                const float v = acc[i] + b;
-                if (m < p.M) {
-                    store_y<O>(p.y, m * p.ldy + n, v);
-                    amax = fmaxf(amax, fabsf(v));
-                }
-            }
-            if (O == Elem::kF16 && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
-        }
+        if (!ok) sum[0] = 0.f;  // the status says that the result is not one
     }
+    // every role is done: the stages' memory now holds the sums [NT][128]
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, S::TMEM_COLS);
+    }
+    float* part = reinterpret_cast<float*>(sA);
+    if (warp >= 4) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) part[i * 128 + threadIdx.x - 128] = sum[i];
+    }
+    if (split > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    // rows [rank NT / split, (rank + 1) NT / split) of the tile, summed over the ranks in order
+    const int col = threadIdx.x & 127, n = n0 + col;
+    const float b = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+    float amax = 0.f;
+    for (int i = rank * (NT / split) + (threadIdx.x >> 7); i < (rank + 1) * (NT / split); i += 2) {
+        if (m0 + i >= p.M || n >= p.N) break;
+        float v = 0.f;
+        if (split == 1) {
+            v = part[i * 128 + col];
+        } else {
+            const uint32_t at = smem_u32(part + i * 128 + col);
+            for (int r = 0; r < split; ++r) v += ld_shared_cluster(mapa_shared(at, r));
+        }
+        v += b;
+        store_y<O>(p.y, (m0 + i) * p.ldy + n, v);
+        amax = fmaxf(amax, fabsf(v));
+    }
+    if (O == Elem::kF16 && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
+    if (split > 1) cluster_sync();  // a CTA's sums are read until here
+}
+
+// ---------------------------------------------------------------------------
+// Large products: persistent CTA pairs (clusters of 2, cta_group::2) on tiles
+// of 256 x BN.  Per k-block the pair's four MMAs fill one of the TMEM
+// accumulators, and the accumulation must read all of it back: at BN = 256 a
+// CTA's 128 x 256 partial takes the tensor core 512 cycles, its reading (the
+// four sub-partitions together 512 bytes a cycle) and its FMAs (128 a cycle)
+// 256 cycles each, so two accumulators and two warps per sub-partition keep
+// the MMAs fed.  Roles (384 threads):
+//   warp 0      TMA producer of its CTA's 128 rows of x and BN / 2 of w;
+//   warp 1      (even CTA) MMA issuer;
+//   warp 2      TMEM allocator;
+//   warp 3      scales: each k-block's 128 row scales and two weight scales
+//               into a ring in shared memory, by asynchronous copies;
+//   warps 4-11  accumulation: warp (4 + 4 h + q) owns rows [32 q, +32) and
+//               columns [h BN / 2, +BN / 2), thread = row, BN / 2 fp32 sums in
+//               registers (the control warps give registers up for them).  A
+//               half of the columns lies within one weight block, so one
+//               factor per thread serves a k-block.
+template <int BN>
+struct WideShape {
+    static constexpr int HALF = BN / 2;
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = HALF * 128;
+    static constexpr int STAGES = BN == 256 ? 5 : 6;
+    static constexpr int ACC = 512 / BN;
+    static constexpr int WARPS = 8;
+    static constexpr int BOXES = 4096;  // a warp's 32 x 32 boxes: one of fp32 or two of 16 bits
+    static constexpr int SR = 8;        // ring of scales, 2 x 128 each
+    static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + WARPS * BOXES + SR * 1024 + 1024 + 512;
+    static constexpr int THREADS = 128 + 32 * WARPS;
+    static constexpr int CONTROL_REGS = 40, SUM_REGS = 232;  // 128 * 40 + 256 * 232 = 384 * 168
+    static_assert(SMEM <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+template <int BN, Elem O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
+    dense_e4m3_wide_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                           const __grid_constant__ CUtensorMap tmY, DenseE4Params p, bool tma_out) {
+    using S = WideShape<BN>;
+    constexpr int STAGES = S::STAGES, ACC = S::ACC, HALF = S::HALF, SR = S::SR;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sA = smem;
+    uint8_t* sB = sA + STAGES * S::A_BYTES;
+    uint8_t* boxes = sB + STAGES * S::B_BYTES;
+    float* sScale = reinterpret_cast<float*>(boxes + S::WARPS * S::BOXES);  // [SR][128 rows, 2 weight blocks]
+    uint64_t* full = reinterpret_cast<uint64_t*>(sScale + SR * 130);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + ACC;
+    uint64_t* cfull = tempty + ACC;
+    uint64_t* cempty = cfull + SR;
+    uint64_t* drain = cempty + SR;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();  // 0: the CTA that issues the MMAs
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int n_tiles = (p.N + BN - 1) / BN;
+    const int num_tiles = (p.M + 255) / 256 * n_tiles;
+    const int kblocks = (p.K + kE4Block - 1) / kE4Block;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < ACC; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], 2 * S::WARPS);  // the accumulation warps of both CTAs
+        }
+        for (int s = 0; s < SR; ++s) {
+            mbar_init(&cfull[s], 32);
+            mbar_init(&cempty[s], S::WARPS);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmW);
+        if (tma_out) tma_prefetch_desc(&tmY);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t full_lead = mapa_shared(smem_u32(full), 0);
+    const uint32_t tempty_lead = mapa_shared(smem_u32(tempty), 0);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CONTROL_REGS));
+        if (warp == 0) {
+            int stage = 0;
+            uint32_t phase = 0, issued = 0, parity = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+                const int row = tile / n_tiles * 256 + static_cast<int>(rank) * 128;
+                const int col = tile % n_tiles * BN + static_cast<int>(rank) * HALF;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (elect_one()) {
+                        // both CTAs' loads complete on the even CTA's barrier
+                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (S::A_BYTES + S::B_BYTES));
+                        tma_load_2d_pair(sA + stage * S::A_BYTES, &tmX, full_lead + 8 * stage, kb * 128, row);
+                        tma_load_2d_pair(sB + stage * S::B_BYTES, &tmW, full_lead + 8 * stage, kb * 128, col);
+                    }
+                    __syncwarp();
+                    issued |= 1u << stage;
+                    parity = (parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // the even CTA sees every load of both CTAs land
+            if (rank == 0)
+                for (int s = 0; s < STAGES; ++s)
+                    if (issued & (1u << s)) mbar_drain(&full[s], (parity >> s) & 1);
+        } else if (warp == 1 && rank == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(256, BN);
+            const uint64_t ad0 = sdesc_k128(smem_u32(sA)), bd0 = sdesc_k128(smem_u32(sB));
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool issued = false, ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1, p.status, abort_flag) ||
+                        !mbar_wait_warp(&full[stage], phase, p.status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t ad = ad0 + stage * (S::A_BYTES / 16), bd = bd0 + stage * (S::B_BYTES / 16);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_f8_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+                        umma_commit_pair_mc(smem_u32(&empty[stage]), 0x3);
+                        umma_commit_pair_mc(smem_u32(&tfull[acc]), 0x3);
+                    }
+                    __syncwarp();
+                    issued = true;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (++acc == ACC) {
+                        acc = 0;
+                        acc_phase ^= 1;
+                    }
+                }
+            }
+            if (issued) {
+                if (elect_one()) umma_commit_pair(smem_u32(drain));
+                mbar_drain(drain, 0);
+            }
+        } else if (warp == 3) {
+            const int nblocks = (p.N + kE4Block - 1) / kE4Block;
+            int slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+                const int row = tile / n_tiles * 256 + static_cast<int>(rank) * 128 + lane;
+                const int nb = (tile % n_tiles * BN + (lane & 1) * HALF) / kE4Block;
+                const bool in_n = nb < nblocks;
+                const float* xs = p.x_scale + row;
+                const float* ws = p.w_scale + (in_n ? static_cast<int64_t>(nb) * kblocks : 0);
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait_warp(&cempty[slot], phase ^ 1, p.status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    float* to = sScale + slot * 130;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {  // rows past the end: zeros
+                        const bool in = row + 32 * i < p.M;
+                        cp_async_f32(to + lane + 32 * i, in ? xs + 32 * i : p.x_scale, in);
+                    }
+                    if (lane < 2) cp_async_f32(to + 128 + lane, ws + kb, in_n);
+                    cp_async_arrive(&cfull[slot]);
+                    xs += p.ld_xs;
+                    if (++slot == SR) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // every copy has landed before the CTA may exit
+            cp_async_wait_all();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SUM_REGS));
+        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+        uint8_t* box = boxes + ew * S::BOXES;
+        const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+        int acc = 0, slot = 0, stores = 0;
+        uint32_t acc_phase = 0, slot_phase = 0;
+        bool ok = true;
+        for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+            const int row0 = tile / n_tiles * 256 + static_cast<int>(rank) * 128 + quarter * 32;
+            const int col0 = tile % n_tiles * BN + half * HALF;
+            const int row = row0 + lane;
+            uint64_t sum[HALF / 2];
+#pragma unroll
+            for (int i = 0; i < HALF / 2; ++i) sum[i] = 0;
+            for (int kb = 0; kb < kblocks; ++kb) {
+                if (!mbar_wait_warp(&cfull[slot], slot_phase, p.status, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                const float s = sScale[slot * 130 + quarter * 32 + lane] * sScale[slot * 130 + 128 + half];
+                const uint64_t s2 = pair_of(s, s);
+                if (!mbar_wait_warp(&tfull[acc], acc_phase, p.status, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ta = tmem + lane_addr + acc * BN + half * HALF;
+                uint32_t t[2][16];
+                tmem_ld16(ta, t[0]);
+#pragma unroll
+                for (int c = 0; c < HALF / 16; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < HALF / 16) {
+                        tmem_ld16(ta + (c + 1) * 16, t[(c + 1) & 1]);
+                    } else {  // all of it is in registers: the next MMAs may have the accumulator
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive_cluster_relaxed(tempty_lead + 8 * acc);
+                            mbar_arrive(&cempty[slot]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        sum[c * 8 + i] =
+                            fma_pair(pair_of(__uint_as_float(t[c & 1][2 * i]), __uint_as_float(t[c & 1][2 * i + 1])), s2,
+                                     sum[c * 8 + i]);
+                }
+                if (++acc == ACC) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
+                if (++slot == SR) {
+                    slot = 0;
+                    slot_phase ^= 1;
+                }
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < HALF / 32; ++c) {
+                const int c0 = col0 + c * 32;
+                if (c0 >= p.N || row0 >= p.M) break;  // warp-uniform
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) split_pair(sum[c * 16 + i], v[2 * i], v[2 * i + 1]);
+                if (p.bias) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c0 + i < p.N) v[i] += __ldg(p.bias + c0 + i);
+                }
+                if (O == Elem::kF16) {
+                    float amax = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
+                    if (row < p.M && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
+                }
+                if (tma_out) {
+                    // the store that last read this box has left it
+                    uint8_t* b = O == Elem::kF32 ? box : box + (stores & 1) * 2048;
+                    if (lane == 0) {
+                        if (O == Elem::kF32) bulk_wait_read<0>();
+                        else bulk_wait_read<1>();
+                    }
+                    __syncwarp();
+                    if constexpr (O == Elem::kF32) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(b + ((lane * 128 + i * 16) ^ ((lane & 7) << 4))) =
+                                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<uint4*>(b + ((lane * 64 + i * 16) ^ (((lane >> 1) & 3) << 4))) =
+                                make_uint4(pack2<O == Elem::kF16>(v[8 * i], v[8 * i + 1]),
+                                           pack2<O == Elem::kF16>(v[8 * i + 2], v[8 * i + 3]),
+                                           pack2<O == Elem::kF16>(v[8 * i + 4], v[8 * i + 5]),
+                                           pack2<O == Elem::kF16>(v[8 * i + 6], v[8 * i + 7]));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmY, b, c0, row0);
+                        bulk_commit();
+                    }
+                    ++stores;
+                } else {
+                    // rows of y that TMA cannot address: through shared memory, so
+                    // that a warp writes 32 neighbours of one row
+                    float* f = reinterpret_cast<float*>(box);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) f[lane * 32 + (i ^ lane)] = v[i];
+                    __syncwarp();
+                    for (int r = 0; r < 32; ++r)
+                        if (row0 + r < p.M && c0 + lane < p.N)
+                            store_y<O>(p.y, (row0 + r) * p.ldy + c0 + lane, f[r * 32 + (lane ^ r)]);
+                    __syncwarp();
+                }
+            }
+        }
+        if (tma_out && lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
     }
 }
 
@@ -235,7 +607,7 @@ cudaError_t allow_smem(K kern, int bytes, unsigned& configured) {
 }
 
 template <int NT, Elem O>
-cudaError_t launch_thin(const DenseE4Params& p, cudaStream_t st) {
+cudaError_t launch_thin(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     using S = ThinShape<NT>;
     static unsigned configured = 0;
     auto kern = dense_e4m3_thin_kernel<NT, O>;
@@ -244,16 +616,76 @@ cudaError_t launch_thin(const DenseE4Params& p, cudaStream_t st) {
     CUtensorMap tw, tx;
     if (!make_kmajor_tmap(&tw, p.wq, 1, p.N, p.K, p.ldw, 128) || !make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, NT))
         return cudaErrorInvalidValue;
-    const dim3 grid((p.N + 127) / 128, (p.M + NT - 1) / NT);
-    return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tw, tx, p);
+    const int tiles_n = (p.N + 127) / 128, tiles_m = (p.M + NT - 1) / NT, kblocks = (p.K + kE4Block - 1) / kE4Block;
+    // K is split over up to eight CTAs while they find room in one wave
+    const int64_t room = static_cast<int64_t>(num_sms) * (NT == 128 ? 1 : 2);
+    int split = 1;
+    while (split < 8 && 2 * split <= kblocks && 2 * split * static_cast<int64_t>(tiles_n) * tiles_m <= room) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles_n * split, tiles_m);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, tw, tx, p, split);
+}
+
+template <int BN, Elem O>
+cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
+    using S = WideShape<BN>;
+    static unsigned configured = 0;
+    auto kern = dense_e4m3_wide_kernel<BN, O>;
+    cudaError_t e = allow_smem(kern, S::SMEM, configured);
+    if (e != cudaSuccess) return e;
+    CUtensorMap tx, tw, ty;
+    if (!make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, 128) ||
+        !make_kmajor_tmap(&tw, p.wq, 1, p.N, p.K, p.ldw, S::HALF))
+        return cudaErrorInvalidValue;
+    const bool tma_out = make_epilogue_tmap(&ty, p.y, O == Elem::kF32, O == Elem::kF16, p.M, p.N, p.ldy);
+    if (!tma_out) ty = tx;  // not read
+    const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
+    // one pair per tile slot: as many as can be resident at once
+    static int resident[32] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int pairs = dev < 32 ? __atomic_load_n(&resident[dev], __ATOMIC_ACQUIRE) : 0;
+    if (pairs == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * (num_sms / 2));
+        cfg.blockDim = dim3(S::THREADS);
+        cfg.dynamicSmemBytes = S::SMEM;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs <= 0) {
+            cudaGetLastError();
+            pairs = num_sms / 2;
+        }
+        if (dev < 32) __atomic_store_n(&resident[dev], pairs, __ATOMIC_RELEASE);
+    }
+    const dim3 grid(2 * static_cast<unsigned>(tiles < pairs ? tiles : pairs));
+    return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tx, tw, ty, p, tma_out);
 }
 
 template <Elem O>
 cudaError_t launch_out(const DenseE4Params& p, int num_sms, cudaStream_t st) {
-    if (p.M <= 16) return launch_thin<16, O>(p, st);
-    if (p.M <= 32) return launch_thin<32, O>(p, st);
-    if (p.M <= 64) return launch_thin<64, O>(p, st);
-    return launch_thin<128, O>(p, st);
+    if (p.M > 256) return launch_wide<256, O>(p, num_sms, st);
+    if (p.M <= 16) return launch_thin<16, O>(p, num_sms, st);
+    if (p.M <= 32) return launch_thin<32, O>(p, num_sms, st);
+    if (p.M <= 64) return launch_thin<64, O>(p, num_sms, st);
+    return launch_thin<128, O>(p, num_sms, st);
 }
 
 }  // namespace
