@@ -297,6 +297,30 @@ int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, c
                   const float *w_scale, const float *bias, void *y, int ldy, int dtype, int M, int N, int K,
                   void *stream, char **err);
 
+/* rg_cross_attention: no counterpart in the reference.  Attention of query
+ * sequences to the keys and values of other sequences, of another length each:
+ * a decoder's or a pooler's tokens over an encoder's states.  q [Tq x ldq] and
+ * out [Tq x ldo] hold the query sequences packed, sequence s in rows [cu_q[s],
+ * cu_q[s + 1]); its keys and values are rows [kv_begin[s], kv_begin[s] +
+ * kv_len[s]) of k [Tk x ldk] and v [Tk x ldv].  So the states may be packed or
+ * padded, several sequences may share one text (beams), and the order is free;
+ * rows outside a sequence's own are not read into its result, whatever they
+ * hold.  Every query sees every key of its sequence; with none (kv_len 0) its
+ * output is zeros.  Rows of out outside every sequence are left alone.
+ *
+ * Heads as in rg_attention: query head h at columns h * head_dim, key/value
+ * head h / (heads / kv_heads); head dims 32, 64, 128, 256; dtype
+ * RG_DTYPE_BF16 or F16 for q, k, v and out; scale positive.  Rows start on
+ * 16-byte boundaries (bases, and strides a multiple of 8).  cu_q [nseq + 1],
+ * kv_begin [nseq], kv_len [nseq] are device arrays, read when the call runs;
+ * max_q and max_kv bound the lengths they hold and choose the kernel.  A
+ * sequence that does not fit the buffers or these bounds is skipped, its output
+ * left alone, and rg_kernel_status reports it.  Deterministic. */
+int rg_cross_attention(const void *q, const void *k, const void *v, int ldq, int ldk, int ldv, const int32_t *cu_q,
+                       const int32_t *kv_begin, const int32_t *kv_len, int nseq, int Tq, int Tk, int max_q,
+                       int max_kv, int heads, int kv_heads, int head_dim, float scale, int dtype, void *out, int ldo,
+                       void *stream, char **err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,7 +25,8 @@ LIB = PKG / "librembed_gpu.so"
 INCLUDE = PKG.parent / "include"
 SOURCES = ["gemm.cu", "gemm_kind_bf16.cu", "gemm_kind_s8.cu", "gemm_kind_f16.cu", "gemm_kind_w8.cu",
            "gemm_kind_tf32x3.cu", "kernels.cu", "attention_tc.cu", "runtime.cu", "noalloc.cu",
-           "kernel_abi.cu", "quant_e4m3.cu", "dense_e4m3.cu"]
+           "kernel_abi.cu", "quant_e4m3.cu", "dense_e4m3.cu", "cross_attention.cu",
+           "cross_attention_rows.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
          "--expt-relaxed-constexpr", f"-I{INCLUDE}"]

@@ -743,8 +743,8 @@ static EncodeTiledFn encode_fn_attn() {
 
 // [rows x cols] 16-bit matrix with row stride ld elements; boxes of 64
 // columns (128 bytes, 128-byte swizzle) x box_rows.
-static bool make_rows_tmap(CUtensorMap* map, const void* base, bool f16, uint64_t rows, uint64_t cols, uint64_t ld,
-                           uint32_t box_rows) {
+bool make_rows_tmap(CUtensorMap* map, const void* base, bool f16, uint64_t rows, uint64_t cols, uint64_t ld,
+                    uint32_t box_rows) {
     EncodeTiledFn fn = encode_fn_attn();
     if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) != 0 || (ld * 2) % 16 != 0) return false;
     cuuint64_t dims[2] = {cols, rows};

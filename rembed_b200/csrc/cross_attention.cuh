@@ -1,0 +1,58 @@
+// cross_attention.cuh - attention of packed query sequences to the keys and
+// values of other sequences (an encoder's states), each of its own length.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rg {
+
+// attention_tc.cu: tensor map over a 16-bit matrix of `rows` x `cols` at row
+// stride ld, boxes of 64 columns (128 bytes, 128-byte swizzle) x box_rows.
+bool make_rows_tmap(CUtensorMap* map, const void* base, bool f16, uint64_t rows, uint64_t cols, uint64_t ld,
+                    uint32_t box_rows);
+
+// Query sequence s: rows [cu_q[s], cu_q[s + 1]) of q and out; its keys and
+// values: rows [kv_begin[s], kv_begin[s] + kv_len[s]) of k and v.  Query head h
+// at columns h * D, key/value head h / group.
+struct CrossParams {
+    const uint16_t *q, *k, *v;
+    bool f16;
+    int ldq, ldk, ldv;
+    const int32_t *cu_q, *kv_begin, *kv_len;
+    int nseq, Tq, Tk, max_q, max_kv;
+    int heads, kv_heads, group;
+    float scale_log2;  // scale * log2(e), positive
+    uint16_t* out;
+    int ldo;
+    int* status;
+};
+
+// One query sequence's part, read on the device; false (with kStatusBadShape
+// raised) if it does not lie within the buffers and the given longest lengths.
+struct CrossSeq {
+    int q0, nq, k0, nk;
+};
+#ifdef __CUDACC__
+__device__ __forceinline__ bool cross_seq(const CrossParams& p, int s, CrossSeq& c, int bad_shape) {
+    c.q0 = __ldg(p.cu_q + s);
+    const int q1 = __ldg(p.cu_q + s + 1);
+    c.k0 = __ldg(p.kv_begin + s);
+    c.nk = __ldg(p.kv_len + s);
+    c.nq = q1 - c.q0;
+    const bool ok = c.q0 >= 0 && q1 >= c.q0 && q1 <= p.Tq && c.nq <= p.max_q && c.nk >= 0 && c.nk <= p.max_kv &&
+                    c.k0 >= 0 && c.k0 <= p.Tk - c.nk;
+    if (!ok && threadIdx.x == 0) atomicOr(p.status, bad_shape);
+    return ok;
+}
+#endif
+
+// Few query rows per key/value head (one or a few tokens): bound by reading K and V.
+cudaError_t launch_cross_rows(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st);
+// Any number of query rows: tiles of 128 on the tensor cores of tcgen05.
+cudaError_t launch_cross_tiles(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st);
+// The one of the two that suits the call.
+cudaError_t launch_cross(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st);
+
+}  // namespace rg

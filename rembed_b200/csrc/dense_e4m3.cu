@@ -463,6 +463,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
             // every copy has landed before the CTA may exit
             cp_async_wait_all();
         }
+        // The control warps gave registers up: nothing is shared with the
+        // accumulation warps' code from here on but the barrier.
+        __syncwarp();
+        tc_fence_before();
+        cluster_sync();
+        if (warp == 2) {
+            tc_fence_after();
+            tmem_dealloc_pair(tmem, 512);
+        }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SUM_REGS));
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
@@ -585,14 +594,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
         }
         if (tma_out && lane == 0) bulk_wait_read<0>();
         __syncwarp();
-    }
-
-    __syncwarp();
-    tc_fence_before();
-    cluster_sync();
-    if (warp == 2) {
-        tc_fence_after();
-        tmem_dealloc_pair(tmem, 512);
+        tc_fence_before();
+        cluster_sync();
     }
 }
 

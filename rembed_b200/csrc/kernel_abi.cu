@@ -1,7 +1,7 @@
 // kernel_abi.cu - kernel-level C ABI entry points beyond the dense
 // projections: varlen attention, the full-int8 row quantiser and integer
-// GEMM, the e4m3 quantisers and block-scaled GEMM, and the status check
-// shared by every kernel-level call.
+// GEMM, the e4m3 quantisers and block-scaled GEMM, cross attention, and the
+// status check shared by every kernel-level call.
 //
 // These calls take device pointers on the current CUDA device and are
 // asynchronous on the caller's stream.  A failure that a kernel detects on
@@ -22,6 +22,7 @@
 #include <string>
 
 #include "rembed_gpu.h"
+#include "cross_attention.cuh"
 #include "e4m3.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
@@ -325,6 +326,74 @@ int rg_dense_e4m3(const uint8_t* xq, int ldx, const float* x_scale, int ld_xs, c
     p.status = status;
     e = rg::launch_dense_e4m3(elem_of(dtype), p, sms, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return set_err(err, "rg_dense_e4m3: launch: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int rg_cross_attention(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv, const int32_t* cu_q,
+                       const int32_t* kv_begin, const int32_t* kv_len, int nseq, int Tq, int Tk, int max_q, int max_kv,
+                       int heads, int kv_heads, int head_dim, float scale, int dtype, void* out, int ldo, void* stream,
+                       char** err) {
+    if (nseq <= 0 || Tq <= 0) return 0;
+    if (!q || !k || !v || !cu_q || !kv_begin || !kv_len || !out) return set_err(err, "rg_cross_attention: null buffer");
+    if (dtype != RG_DTYPE_BF16 && dtype != RG_DTYPE_F16)
+        return set_err(err, "rg_cross_attention: dtype %d unsupported (bf16 or fp16)", dtype);
+    if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return set_err(err, "rg_cross_attention: head dim %d unsupported (32, 64, 128 or 256)", head_dim);
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || heads > 65535)
+        return set_err(err, "rg_cross_attention: heads %d not a multiple of kv_heads %d, or over 65535", heads, kv_heads);
+    const int64_t qd = static_cast<int64_t>(heads) * head_dim, kvd = static_cast<int64_t>(kv_heads) * head_dim;
+    if (ldq < qd || ldo < qd || ldk < kvd || ldv < kvd)
+        return set_err(err, "rg_cross_attention: a row stride is narrower than its heads");
+    if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(out, 16) || ldq % 8 != 0 ||
+        ldk % 8 != 0 || ldv % 8 != 0 || ldo % 8 != 0)
+        return set_err(err, "rg_cross_attention: rows must start on 16-byte boundaries");
+    if (misaligned(cu_q, 4) || misaligned(kv_begin, 4) || misaligned(kv_len, 4))
+        return set_err(err, "rg_cross_attention: a table is not aligned to its type");
+    if (Tk <= 0 || max_q <= 0 || max_kv < 0)
+        return set_err(err, "rg_cross_attention: Tk=%d and max_q=%d must be positive, max_kv=%d not negative", Tk, max_q,
+                       max_kv);
+    if (!(scale > 0.f && scale <= 3.0e38f)) return set_err(err, "rg_cross_attention: scale must be positive and finite");
+    const int group = heads / kv_heads;
+    max_q = std::min(max_q, Tq);
+    max_kv = std::min(max_kv, Tk);
+    // a sequence's grid: at most 8 CTAs for each 16 rows or key/value head, or for each 128 rows
+    if (static_cast<int64_t>(nseq) * ((max_q + 127) / 128) > 0x7fffffff / 8)
+        return set_err(err, "rg_cross_attention: %d sequences of up to %d queries are too many for one call", nseq, max_q);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return set_err(err, "cudaGetDevice: %s", cudaGetErrorString(e));
+    int sms = 148;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return set_err(err, "cudaDeviceGetAttribute: %s", cudaGetErrorString(e));
+    int* status = nullptr;
+    e = rg::kernel_status_word(dev, &status);
+    if (e != cudaSuccess) return set_err(err, "rg_cross_attention: status word: %s", cudaGetErrorString(e));
+    rg::CrossParams p{};
+    p.q = static_cast<const uint16_t*>(q);
+    p.k = static_cast<const uint16_t*>(k);
+    p.v = static_cast<const uint16_t*>(v);
+    p.f16 = dtype == RG_DTYPE_F16;
+    p.ldq = ldq;
+    p.ldk = ldk;
+    p.ldv = ldv;
+    p.cu_q = cu_q;
+    p.kv_begin = kv_begin;
+    p.kv_len = kv_len;
+    p.nseq = nseq;
+    p.Tq = Tq;
+    p.Tk = Tk;
+    p.max_q = max_q;
+    p.max_kv = max_kv;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.group = group;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.out = static_cast<uint16_t*>(out);
+    p.ldo = ldo;
+    p.status = status;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    e = rg::launch_cross(p, head_dim, sms, st);
+    if (e != cudaSuccess) return set_err(err, "rg_cross_attention: launch: %s", cudaGetErrorString(e));
     return 0;
 }
 

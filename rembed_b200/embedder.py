@@ -129,6 +129,10 @@ SIGNATURES = {
                                              ctypes.c_int, _VP, ctypes.c_int, _VP, _ERR]),
     "rg_quantize_tiles_e4m3": (ctypes.c_int, [_VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
                                               ctypes.c_int, _VP, _VP, _ERR]),
+    "rg_cross_attention": (ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP, _VP, _VP,
+                                          ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                          ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int, _VP,
+                                          ctypes.c_int, _VP, _ERR]),
     "rg_dense_e4m3": (ctypes.c_int, [_VP, ctypes.c_int, _VP, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP, _VP,
                                      ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP,
                                      _ERR]),
