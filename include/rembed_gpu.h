@@ -272,8 +272,9 @@ int rg_dense_s8(const int8_t *xq, const float *row_scale, const int8_t *wq, cons
  * F16 or BF16) -> q [M x K] e4m3 bytes (row stride ldq; columns from K on are
  * left alone) and scale[b * ld_scale + m] for block b of row m, b <
  * ceil(K / 128), ld_scale >= M.  scale = maxabs(block) / 448 (1 for a block
- * of zeros, at least 2^-126), q = e4m3(x * (1 / scale)), to nearest, ties to
- * even, clamped to +-448.  A block with a NaN or an infinity stands for NaNs.
+ * of zeros, at least 2^-126), q = the e4m3 value next to 448 x / maxabs(block)
+ * (x / 2^-126 where the scale is that), ties to even, rounded once from the
+ * exact quotient.  A block with a NaN or an infinity stands for NaNs.
  * rg_dense_e4m3 reads q with ldq a multiple of 16 from a 16-byte aligned
  * base.
  *

@@ -2,19 +2,27 @@
 //
 // A block is 128 values of one row (activations) or a tile of 128 x 128
 // (weights).  With a = max |x| over the block,
-//     s = a / 448      (1 for a block of zeros, never below 2^-126)
-//     q = e4m3(x * (1 / s)), to nearest, ties to even, clamped to +-448
-// so that q * s is within half an e4m3 step of x.  The maximum is taken on the
-// bit patterns of |x| as unsigned integers, where a NaN orders above infinity:
-// a block with a NaN gets the scale NaN, one with an infinity the scale
-// infinity (then x * 0 is NaN for the infinity and 0 elsewhere, and 0 * inf
-// is NaN), so a block that held either is NaN all over once it is scaled back.
+//     scale = a / 448   (1 for a block of zeros, never below 2^-126)
+//     q = the e4m3 value next to 448 x / a, ties to even
+// (next to x / 2^-126 where the scale is that).  The quotient is rounded once,
+// from its exact value: a product with a rounded reciprocal would put values
+// on the wrong side of a tie, and with 16-bit inputs exact ties are common.
+// With r + d = 448 / a (r the quotient towards zero, d its remainder's, both
+// once per block) and y = x r rounded, y + ((x r - y) + x d) is the quotient to
+// some 2^-47 of itself.  16-bit x and a cannot come nearer to a tie than 2^-18
+// without being one, so there its nearest float says all.  For fp32 the
+// products with r (1 -+ 2^-22) enclose it, and where both round to the same
+// bytes that is the answer; else the sum is cut to a float whose last bit is
+// set if anything was cut off, which four bits' rounding cannot mistake for a
+// tie.
+// A NaN in a block makes the scale NaN, an infinity makes it infinite (with
+// r = d = 0: the infinity becomes NaN, the others 0, and 0 * inf is NaN): a
+// block that held either is NaN all over once it is scaled back.
 //
 // Both kernels are bound by HBM: each value is read once into registers, the
 // maximum is found there, and one byte is written.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "act16.cuh"
 #include "e4m3.cuh"
@@ -22,6 +30,31 @@
 
 namespace rg {
 namespace {
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// x (r + d) rounded so that its rounding to e4m3 is that of the exact product.
+__device__ __forceinline__ float scaled16(float x, float2 inv) {
+    const float y = x * inv.x;
+    return y + __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y));
+}
+__device__ __forceinline__ float scaled32(float x, float2 inv) {
+    const float y = __fmul_rz(x, inv.x);
+    const float e = __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y));
+    const float cut = __fadd_rz(y, e);
+    return __uint_as_float(__float_as_uint(cut) | (e != cut - y ? 1u : 0u));
+}
+
+// Two values as e4m3, to nearest, ties to even, clamped to +-448; the first in the low byte.
+__device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
 
 // One lane's 16 bytes of a block's row: V values, LANES lanes a row.
 template <Elem E>
@@ -60,28 +93,39 @@ struct Lane {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // max |x| of the V values, NaN if one is (as bits, which order like the values)
     static __device__ __forceinline__ uint32_t max_bits(const uint4& u) {
         float f[V];
         unpack(u, f);
-        uint32_t m = 0u;
+        float m = fabsf(f[0]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-        return m;
+        for (int i = 1; i < V; ++i) m = max_nan(m, fabsf(f[i]));
+        return __float_as_uint(m);
     }
-    // The V values times inv as e4m3 bytes to columns c.. of a row.
-    static __device__ __forceinline__ void store(uint8_t* row, int c, int K, bool vec, const uint4& u, float inv) {
-        if (c >= K) return;
+    // The V values over their scale as e4m3 bytes.
+    static __device__ __forceinline__ void convert(const uint4& u, float2 inv, uint32_t (&w)[V / 4]) {
         float f[V];
         unpack(u, f);
-        uint32_t w[V / 4];
+        if constexpr (E == Elem::kF32) {
+            // between these two products lies the exact one; a tie between them is rare
+            const float lo = inv.x * (1.0f - 0x1p-22f), hi = inv.x * (1.0f + 0x1p-22f);
+            w[0] = to_e4m3x2(f[0] * lo, f[1] * lo) | to_e4m3x2(f[2] * lo, f[3] * lo) << 16;
+            const uint32_t v = to_e4m3x2(f[0] * hi, f[1] * hi) | to_e4m3x2(f[2] * hi, f[3] * hi) << 16;
+            if (w[0] == v) return;
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-            const uint32_t lo =
-                __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi =
-                __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-            w[i] = lo | (hi << 16);
+            for (int i = 0; i < V; ++i) f[i] = scaled32(f[i], inv);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = scaled16(f[i], inv);
         }
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            w[i] = to_e4m3x2(f[4 * i], f[4 * i + 1]) | to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16;
+    }
+    static __device__ __forceinline__ void store(uint8_t* row, int c, int K, bool vec, const uint4& u, float2 inv) {
+        if (c >= K) return;
+        uint32_t w[V / 4];
+        convert(u, inv, w);
         if (vec && c + V <= K) {
             if constexpr (V == 8)
                 *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
@@ -95,22 +139,90 @@ struct Lane {
     }
 };
 
-__device__ __forceinline__ float block_scale(uint32_t max_bits) {
-    if (max_bits == 0u) return 1.0f;
-    const float s = __uint_as_float(max_bits) / kE4Max;
-    return s < 1.17549435e-38f ? 1.17549435e-38f : s;  // a NaN stays
+// A block's scale and its reciprocal (r, d) from the bits of its maximum.
+__device__ __forceinline__ float block_scale(uint32_t max_bits, float2& inv) {
+    const float a = __uint_as_float(max_bits);
+    constexpr float kLeast = 1.17549435e-38f;  // 2^-126
+    if (a == 0.f) {
+        inv = make_float2(1.f, 0.f);
+        return 1.f;
+    }
+    const float s = a / kE4Max;
+    if (s < kLeast) {
+        inv = make_float2(8.507059e37f, 0.f);  // 2^126
+        return kLeast;
+    }
+    const float r = __fdiv_rz(kE4Max, a);
+    inv = make_float2(r, isinf(a) ? 0.f : __fmaf_rn(-r, a, kE4Max) / a);  // a NaN stays
+    return s;
 }
 
-// A warp takes one block column of kGroup warp-wide loads of rows: 8 rows of
-// float32, 16 of a 16-bit type.  All loads are in flight before the first
-// maximum, and the rows' scales, neighbours in memory, leave in one store of
-// at least a 32-byte sector.
-constexpr int kGroup = 8;
+// A warp takes one block column of eight rows (float32: eight warp-wide loads,
+// 16-bit: four).  All loads are in flight before the first maximum, and the
+// rows' scales, neighbours in memory, leave as one 32-byte sector.
+template <Elem E>
+constexpr int kGroup = 8 / Lane<E>::ROWS;
 constexpr int kRowWarps = 8;
+
+template <Elem E, bool FULL>
+__device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int64_t first, int b, int lane, bool vec_x,
+                                                    bool vec_q) {
+    using L = Lane<E>;
+    const int rows = FULL ? 8
+                          : static_cast<int>(min(static_cast<int64_t>(8), p.rows - first));
+    const int c = b * kE4Block + (lane % L::LANES) * L::V;
+    const int mine = lane / L::LANES;  // row of the warp-wide load
+    const uint8_t* src = static_cast<const uint8_t*>(p.x) + (first + mine) * p.ldx * L::BYTES;
+    uint8_t* dst = p.q + (first + mine) * p.ldq;
+    const int64_t src_step = L::ROWS * p.ldx * L::BYTES, dst_step = L::ROWS * p.ldq;
+    uint4 u[kGroup<E>];
+#pragma unroll
+    for (int i = 0; i < kGroup<E>; ++i) {
+        if constexpr (FULL) {
+            u[i] = __ldg(reinterpret_cast<const uint4*>(src + i * src_step + c * L::BYTES));
+        } else {
+            u[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (i * L::ROWS + mine < rows) u[i] = L::load(src + i * src_step, c, p.K, vec_x);
+        }
+    }
+    // lane `row of the group` takes that row's maximum through the divisions
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kGroup<E>; ++i) {
+        uint32_t m = L::max_bits(u[i]);
+        if constexpr (L::ROWS == 1) {
+            m = __reduce_max_sync(0xffffffffu, m);
+            top = lane == i ? m : top;
+        } else {
+#pragma unroll
+            for (int o = L::LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, m, L::LANES);
+            if (lane / 2 == i) top = (lane & 1) == mine ? m : other;
+        }
+    }
+    float2 inv;
+    const float s = block_scale(top, inv);
+    if (lane < rows) p.scale[b * p.ld_scale + first + lane] = s;
+#pragma unroll
+    for (int i = 0; i < kGroup<E>; ++i) {
+        const float2 f = make_float2(__shfl_sync(0xffffffffu, inv.x, i * L::ROWS + mine),
+                                     __shfl_sync(0xffffffffu, inv.y, i * L::ROWS + mine));
+        if constexpr (FULL) {
+            uint32_t w[L::V / 4];
+            L::convert(u[i], f, w);
+            if constexpr (L::V == 8)
+                *reinterpret_cast<uint2*>(dst + i * dst_step + c) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t*>(dst + i * dst_step + c) = w[0];
+        } else {
+            if (i * L::ROWS + mine < rows) L::store(dst + i * dst_step, c, p.K, vec_q, u[i], f);
+        }
+    }
+}
 
 template <Elem E>
 __global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(QuantE4Params p, bool vec_x, bool vec_q) {
-    using L = Lane<E>;
+    constexpr int kRowsOf = 8;
     pdl_trigger();
     pdl_wait();
     const int kb = (p.K + kE4Block - 1) / kE4Block;
@@ -118,53 +230,37 @@ __global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(Quan
     const int64_t item = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
     const int64_t group = item / kb;
     const int b = static_cast<int>(item - group * kb);
-    const int64_t r0 = group * (kGroup * L::ROWS) + lane / L::LANES;
-    if (r0 - lane / L::LANES >= p.rows) return;
-    const int c = b * kE4Block + (lane % L::LANES) * L::V;
-    uint4 u[kGroup];
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-        const int64_t r = r0 + i * L::ROWS;
-        u[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < p.rows) u[i] = L::load(static_cast<const uint8_t*>(p.x) + r * p.ldx * L::BYTES, c, p.K, vec_x);
-    }
-    float mine = 1.0f;  // the scale this lane stores: row `lane` of the group
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-        uint32_t m = L::max_bits(u[i]);
-#pragma unroll
-        for (int o = L::LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float s = block_scale(m);
-        const int64_t r = r0 + i * L::ROWS;
-        if (r < p.rows) L::store(p.q + r * p.ldq, c, p.K, vec_q, u[i], 1.0f / s);
-#pragma unroll
-        for (int j = 0; j < L::ROWS; ++j) {
-            const float sj = __shfl_sync(0xffffffffu, s, j * L::LANES);
-            if (lane == i * L::ROWS + j) mine = sj;
-        }
-    }
-    const int64_t r = group * (kGroup * L::ROWS) + lane;
-    if (lane < kGroup * L::ROWS && r < p.rows) p.scale[b * p.ld_scale + r] = mine;
+    const int64_t first = group * kRowsOf;
+    if (first >= p.rows) return;
+    if (vec_x && vec_q && first + kRowsOf <= p.rows && (b + 1) * kE4Block <= p.K)
+        quantize_rows_group<E, true>(p, first, b, lane, true, true);
+    else
+        quantize_rows_group<E, false>(p, first, b, lane, vec_x, vec_q);
 }
 
-// One CTA per 128 x 128 tile, held in registers (64 bytes of a row's block a
-// warp-wide load, 16 or 8 loads a thread).
-template <Elem E>
-__global__ void __launch_bounds__(256) quantize_tiles_e4m3_kernel(QuantE4Params p, bool vec_x, bool vec_q) {
+// One CTA per 128 x 128 tile, held in registers.
+constexpr int kTileWarps = 16;
+
+template <Elem E, bool FULL>
+__device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t first, int col0, bool vec_x, bool vec_q) {
     using L = Lane<E>;
-    constexpr int LOADS = kE4Block / (8 * L::ROWS);
-    __shared__ uint32_t part[8];
-    pdl_trigger();
-    pdl_wait();
+    constexpr int LOADS = kE4Block / (kTileWarps * L::ROWS);
+    __shared__ uint32_t part[kTileWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = blockIdx.x * kE4Block + (lane % L::LANES) * L::V;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kE4Block + warp * L::ROWS + lane / L::LANES;
+    const int c = col0 + (lane % L::LANES) * L::V;
+    const int64_t r0 = first + warp * L::ROWS + lane / L::LANES;
+    const uint8_t* src = static_cast<const uint8_t*>(p.x) + r0 * p.ldx * L::BYTES;
+    uint8_t* dst = p.q + r0 * p.ldq;
+    const int64_t src_step = kTileWarps * L::ROWS * p.ldx * L::BYTES, dst_step = kTileWarps * L::ROWS * p.ldq;
     uint4 u[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int64_t r = r0 + i * 8 * L::ROWS;
-        u[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < p.rows) u[i] = L::load(static_cast<const uint8_t*>(p.x) + r * p.ldx * L::BYTES, c, p.K, vec_x);
+        if constexpr (FULL) {
+            u[i] = __ldg(reinterpret_cast<const uint4*>(src + i * src_step + c * L::BYTES));
+        } else {
+            u[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r0 + i * kTileWarps * L::ROWS < p.rows) u[i] = L::load(src + i * src_step, c, p.K, vec_x);
+        }
     }
     uint32_t m = 0u;
 #pragma unroll
@@ -172,16 +268,35 @@ __global__ void __launch_bounds__(256) quantize_tiles_e4m3_kernel(QuantE4Params 
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) part[warp] = m;
     __syncthreads();
-    m = part[lane & 7];
-    m = __reduce_max_sync(0xffffffffu, m);
-    const float s = block_scale(m);
-    const float inv = 1.0f / s;
+    m = __reduce_max_sync(0xffffffffu, part[lane & (kTileWarps - 1)]);
+    float2 inv;
+    const float s = block_scale(m, inv);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int64_t r = r0 + i * 8 * L::ROWS;
-        if (r < p.rows) L::store(p.q + r * p.ldq, c, p.K, vec_q, u[i], inv);
+        if constexpr (FULL) {
+            uint32_t w[L::V / 4];
+            L::convert(u[i], inv, w);
+            if constexpr (L::V == 8)
+                *reinterpret_cast<uint2*>(dst + i * dst_step + c) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t*>(dst + i * dst_step + c) = w[0];
+        } else {
+            if (r0 + i * kTileWarps * L::ROWS < p.rows) L::store(dst + i * dst_step, c, p.K, vec_q, u[i], inv);
+        }
     }
     if (threadIdx.x == 0) p.scale[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+}
+
+template <Elem E>
+__global__ void __launch_bounds__(32 * kTileWarps) quantize_tiles_e4m3_kernel(QuantE4Params p, bool vec_x, bool vec_q) {
+    pdl_trigger();
+    pdl_wait();
+    const int64_t first = static_cast<int64_t>(blockIdx.y) * kE4Block;
+    const int col0 = blockIdx.x * kE4Block;
+    if (vec_x && vec_q && first + kE4Block <= p.rows && col0 + kE4Block <= p.K)
+        quantize_tile<E, true>(p, first, col0, true, true);
+    else
+        quantize_tile<E, false>(p, first, col0, vec_x, vec_q);
 }
 
 template <Elem E>
@@ -196,8 +311,7 @@ bool aligned_q(const QuantE4Params& p) {
 template <Elem E>
 cudaError_t rows_of(const QuantE4Params& p, cudaStream_t st) {
     const int64_t kb = (p.K + kE4Block - 1) / kE4Block;
-    const int64_t rows = kGroup * Lane<E>::ROWS;
-    const int64_t warps = (p.rows + rows - 1) / rows * kb;
+    const int64_t warps = (static_cast<int64_t>(p.rows) + 7) / 8 * kb;
     const int64_t grid = (warps + kRowWarps - 1) / kRowWarps;
     if (grid > 0x7fffffff) return cudaErrorInvalidValue;
     return launch_pdl(quantize_rows_e4m3_kernel<E>, dim3(static_cast<unsigned>(grid)), dim3(32 * kRowWarps), 0, st, p,
@@ -208,7 +322,7 @@ template <Elem E>
 cudaError_t tiles_of(const QuantE4Params& p, cudaStream_t st) {
     const dim3 grid((p.K + kE4Block - 1) / kE4Block, (p.rows + kE4Block - 1) / kE4Block);
     if (grid.y > 65535) return cudaErrorInvalidValue;
-    return launch_pdl(quantize_tiles_e4m3_kernel<E>, grid, dim3(256), 0, st, p, aligned_x<E>(p), aligned_q<E>(p));
+    return launch_pdl(quantize_tiles_e4m3_kernel<E>, grid, dim3(32 * kTileWarps), 0, st, p, aligned_x<E>(p), aligned_q<E>(p));
 }
 
 }  // namespace

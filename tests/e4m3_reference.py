@@ -29,6 +29,15 @@ def encode(v):
     return byte.astype(np.uint8)
 
 
+def encode_exact(v):
+    """encode() of extended-precision values: cut to float64 with what is cut off in the last bit, so that no tie
+    is made of a value beside one."""
+    d = v.astype(np.float64)
+    rest = v - d.astype(np.longdouble)
+    low = np.where(rest < 0, np.nextafter(d, -np.inf), np.where(rest > 0, np.nextafter(d, np.inf), d))
+    return encode(np.where(np.isfinite(d) & (rest != 0), low, d))
+
+
 def scale_of(amax):
     """float32 scale of blocks with these maxima."""
     amax = np.asarray(amax, dtype=np.float32)
@@ -49,10 +58,15 @@ def quantize(x, tall):
     """x float32 [rows x K] -> (bytes [rows x K], scales [row blocks x K blocks]); `tall` rows share a scale."""
     rows, K = x.shape
     f = _blocks(x, tall)
-    with np.errstate(invalid="ignore", over="ignore"):
-        s = scale_of(np.abs(f).max(axis=(1, 3)))  # a NaN propagates
-        inv = (np.float32(1) / s).astype(np.float32)
-        q = encode((f * inv[:, None, :, None]).astype(np.float32))
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        amax = np.abs(f).max(axis=(1, 3))  # a NaN propagates
+        s = scale_of(amax)
+        # the exact quotient 448 x / amax, in extended precision (the product is exact; the quotient keeps 64 bits,
+        # and one that is no tie is at least 2^-50 of itself away from one)
+        least, x = s == np.float32(2.0**-126), f.astype(np.longdouble)
+        over = np.where(least | (amax == 0), np.longdouble(1), amax.astype(np.longdouble))
+        by = np.where(least, np.longdouble(2.0**126), np.where(amax == 0, np.longdouble(1), np.longdouble(448)))
+        q = encode_exact(x * by[:, None, :, None] / over[:, None, :, None])
     return q.reshape(f.shape[0] * tall, -1)[:rows, :K], s
 
 
