@@ -2,24 +2,29 @@
 // tiles of 128 query rows of one (sequence, query head) against blocks of BKV
 // keys, one pass with the running maximum and sum of the softmax.
 //
-// Roles (head dims up to 128: two tiles a CTA, 384 threads; 256: one, 256):
-//   warp 0     TMA producer: the query tiles once, then K and V blocks through
-//              two stages each.  In the last block, which may reach past the
-//              sequence's end, the rows of V behind it that share a
-//              16-key MMA step with it are overwritten with zeros (they may
-//              hold anything: 0 * NaN would reach the output);
+// A CTA stays on its SM and walks items of NT tiles (head dims up to 128: two,
+// 384 threads; 256: one, 256 threads), the next item's loads and first
+// products under the last softmax and the output of the one before.  Roles:
+//   warp 0     TMA producer: the query tiles of an item, K and V blocks through
+//              two stages each.  In a text's last block the rows of V behind its
+//              end that share a 16-key MMA step with it are overwritten with
+//              zeros (they may hold anything: 0 * NaN would reach the output);
 //   warp 1     MMA issuer: S = Q K^T into tensor memory, O += P V with P read
-//              from tensor memory, where it takes the place of its S;
+//              from tensor memory, where it takes the place of its S (up to
+//              head dim 128 in two halves, the first under the exponentials of
+//              the second);
 //   warp 2     TMEM allocator;
 //   warps 4..  softmax, four warps a tile, thread = query row = TMEM lane.
 // With two tiles the softmax of one runs under the MMAs of the other; the one
 // tile of head dim 256 has two S buffers instead.  The tensor core finishes a
 // thread's MMAs in order, so a block's S being ready implies that the tile's
 // earlier P V (two tiles: all of them; one tile: all but the last) are done.
-// Few CTAs split the keys over a cluster of up to eight and join their parts
-// through distributed shared memory in rank order.
+// Few items split the keys over a cluster of up to eight CTAs and join their
+// parts through distributed shared memory in rank order.
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "act16.cuh"
 #include "cross_attention.cuh"
@@ -31,14 +36,13 @@ namespace {
 
 template <int D>
 struct TileShape {
-    static constexpr int NT = D == 256 ? 1 : 2;     // query tiles of a CTA
+    static constexpr int NT = D == 256 ? 1 : 2;     // query tiles of an item
     static constexpr int NS = D == 256 ? 2 : 1;     // S buffers of a tile
     static constexpr int BKV = D == 256 ? 64 : 128;  // keys of a block
     static constexpr int QB = D < 64 ? 1 : D / 64;  // 64-column boxes of a row
     static constexpr int Q_BYTES = 128 * QB * 128;
     static constexpr int KV_BYTES = BKV * QB * 128;
-    static constexpr int ST = 2;  // stages of K, and of V
-    static constexpr int LOAD = NT * Q_BYTES + 2 * ST * KV_BYTES;
+    static constexpr int LOAD = NT * Q_BYTES + 4 * KV_BYTES;  // Q, two stages of K and of V
     static constexpr int PART = NT * D * 512;  // a CTA's fp32 outputs, when keys are split
     static constexpr int RING = LOAD > PART ? LOAD : PART;
     static constexpr int SMEM = RING + 2 * NT * 512 + 1024 + 256;
@@ -46,77 +50,127 @@ struct TileShape {
     static constexpr uint32_t O_COL(int t) { return NT * NS * BKV + t * D; }
     static constexpr uint32_t TMEM_COLS = NT * NS * BKV + NT * D <= 256 ? 256 : 512;
     static constexpr int THREADS = 128 + 128 * NT;
+    // keys whose P is handed over before the rest of their block
+    static constexpr int CUT = D == 256 ? BKV : BKV / 2;
     static_assert(NT * NS * BKV + NT * D <= 512 && SMEM <= 232448, "on-chip memory");
 };
 
-// registers of the two-tile kernel: 128 * 80 + 256 * 208 <= 384 * 168
-constexpr int kControlRegs = 80, kSoftmaxRegs = 208;
+template <int N>
+struct Const {
+    static constexpr int value = N;
+};
+
+// registers of the two-tile kernel: 128 * 96 + 256 * 200 <= 384 * 168
+constexpr int kControlRegs = 96, kSoftmaxRegs = 200;
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Pairs of floats in one 64-bit register: half the instructions.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// The largest of three, NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+
+// One item: up to NT tiles of one (sequence, query head), and this CTA's blocks
+// of the sequence's keys.
+struct Work {
+    int h, row, rows;  // query head; first row of q and out; rows from there to the sequence's end
+    int nt;            // tiles with rows
+    int k0, nb;        // first row of k and v, blocks of keys
+    int tail;          // keys of the text's last block
+    bool last;         // the last of the nb blocks is the text's last
+    bool clear;        // and ends within a 16-key step
+};
+
+template <int D>
+__device__ __forceinline__ bool work_of(const CrossParams& p, int item, int qtiles, int rank, int split, bool report,
+                                        Work& w) {
+    using S = TileShape<D>;
+    const int qt = item % qtiles, sh = item / qtiles;
+    w.h = sh % p.heads;
+    CrossSeq c;
+    if (!cross_seq(p, sh / p.heads, c, report ? kStatusBadShape : 0)) return false;
+    const int q0 = qt * (128 * S::NT);
+    w.row = c.q0 + q0;
+    w.rows = c.nq - q0;
+    if (w.rows <= 0) return false;
+    w.nt = min(S::NT, (w.rows + 127) / 128);
+    const int blocks = (c.nk + S::BKV - 1) / S::BKV;
+    const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / split);
+    const int b1 = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split);
+    w.k0 = c.k0 + b0 * S::BKV;
+    w.nb = b1 - b0;
+    w.tail = c.nk - (blocks - 1) * S::BKV;
+    w.last = w.nb > 0 && b1 == blocks;
+    w.clear = w.last && (w.tail & 15) != 0;
+    return true;
 }
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     cross_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, CrossParams p, int split, int qtiles) {
+                       const __grid_constant__ CUtensorMap tmV, CrossParams p, int split, int qtiles, int items) {
     using S = TileShape<D>;
-    constexpr int NT = S::NT, NS = S::NS, BKV = S::BKV, QB = S::QB, ST = S::ST;
+    constexpr int NT = S::NT, NS = S::NS, BKV = S::BKV, QB = S::QB;
+    constexpr int STEPS = BKV / 16, CUT = S::CUT / 16;  // MMA steps of a block, and before the cut
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sQ = smem;                       // [NT][Q_BYTES]
-    uint8_t* sK = sQ + NT * S::Q_BYTES;       // [ST][KV_BYTES]
-    uint8_t* sV = sK + ST * S::KV_BYTES;      // [ST][KV_BYTES]
+    uint8_t* sQ = smem;                    // [NT][Q_BYTES]
+    uint8_t* sK = sQ + NT * S::Q_BYTES;    // [2][KV_BYTES]
+    uint8_t* sV = sK + 2 * S::KV_BYTES;    // [2][KV_BYTES]
     float* sM = reinterpret_cast<float*>(smem + S::RING);  // [NT][128] maximum, then [NT][128] sum
     float* sL = sM + NT * 128;
     uint64_t* qfull = reinterpret_cast<uint64_t*>(sL + NT * 128);
-    uint64_t* kfull = qfull + 1;
-    uint64_t* kempty = kfull + ST;
-    uint64_t* vfull = kempty + ST;
-    uint64_t* vempty = vfull + ST;
-    uint64_t* vfixed = vempty + ST;
-    uint64_t* sfull = vfixed + 1;         // [NT][NS]
-    uint64_t* pfull = sfull + NT * NS;    // [NT]
-    uint64_t* ofull = pfull + NT;         // [NT]
+    uint64_t* qempty = qfull + 1;
+    uint64_t* kfull = qempty + 1;         // [2]
+    uint64_t* kempty = kfull + 2;         // [2]
+    uint64_t* vfull = kempty + 2;         // [2]
+    uint64_t* vempty = vfull + 2;         // [2]
+    uint64_t* vfixed = vempty + 2;        // [2]: of a stage, so that none runs ahead of its reader
+    uint64_t* sfull = vfixed + 2;         // [NT][NS]
+    uint64_t* pfull = sfull + NT * NS;    // [NT][2]: before and after the cut
+    uint64_t* ofull = pfull + NT * 2;     // [NT]
     uint64_t* drain = ofull + NT;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    pdl_wait();  // the sequence table may come from the previous kernel
-    const int rank = blockIdx.x % split, rest = blockIdx.x / split;
-    const int s = rest / qtiles, h = blockIdx.y, hk = h / p.group;
-    const int q0 = rest % qtiles * (128 * NT);
-    CrossSeq c;
-    if (!cross_seq(p, s, c, kStatusBadShape)) return;  // the same for every CTA of a cluster
-    if (q0 >= c.nq) return;
-    const int nt = min(NT, (c.nq - q0 + 127) / 128);
-    const int blocks = (c.nk + BKV - 1) / BKV;
-    // this CTA's share of the key blocks
-    const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / split);
-    const int nb = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split) - b0;
-
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(qfull, 1);
-        for (int i = 0; i < ST; ++i) {
+        mbar_init(qempty, 1);
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&kfull[i], 1);
             mbar_init(&kempty[i], 1);
             mbar_init(&vfull[i], 1);
             mbar_init(&vempty[i], 1);
+            mbar_init(&vfixed[i], 1);
         }
-        mbar_init(vfixed, 1);
         for (int i = 0; i < NT * NS; ++i) mbar_init(&sfull[i], 1);
-        for (int t = 0; t < NT; ++t) {
-            mbar_init(&pfull[t], 4);  // one arrival per softmax warp
-            mbar_init(&ofull[t], 1);
-        }
+        for (int i = 0; i < NT * 2; ++i) mbar_init(&pfull[i], 4);  // one arrival per softmax warp
+        for (int t = 0; t < NT; ++t) mbar_init(&ofull[t], 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -132,139 +186,198 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     __syncthreads();
     tc_fence_after();
     pdl_trigger();  // after the allocation: the next kernel's must not come between
+    pdl_wait();
     const uint32_t tmem = *tmem_slot;
-    // keys of the last block, and whether the MMA step at its end has rows to clear
-    const int tail = c.nk - (blocks - 1) * BKV;
-    const bool last_here = nb > 0 && b0 + nb == blocks;
-    const bool clear = last_here && (tail & 15) != 0;
+    const int rank = blockIdx.x % split;
+    const int first = blockIdx.x / split, stride = gridDim.x / split;
 
     if (warp < 4) {
         if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
-        if (warp == 0 && nb > 0) {
+        if (warp == 0) {
             // ---------------- TMA producer ----------------
-            int ki = 0, vi = 0;  // blocks loaded
-            if (elect_one()) {
-                mbar_arrive_expect_tx(qfull, nt * S::Q_BYTES);
-                for (int t = 0; t < nt; ++t)
-                    for (int b = 0; b < QB; ++b)
-                        tma_load_2d(sQ + t * S::Q_BYTES + b * 16384, &tmQ, qfull, h * D + b * 64, c.q0 + q0 + 128 * t);
-            }
-            __syncwarp();
-            for (int i = 0; i < nb; ++i) {
-                const int st = i % ST, row = c.k0 + (b0 + i) * BKV;
-                const uint32_t ph = (i / ST) & 1;
-                if (!mbar_wait_warp(&kempty[st], ph ^ 1, p.status, abort_flag)) break;
+            uint32_t qn = 0, kn = 0, vn = 0;  // items, blocks of K and blocks of V loaded
+            bool ok = true;
+            for (int item = first; item < items && ok; item += stride) {
+                Work w;
+                if (!work_of<D>(p, item, qtiles, rank, split, lane == 0, w) || w.nb == 0) continue;
+                const int hk = w.h / p.group;
+                ok = mbar_wait_warp(qempty, (qn & 1) ^ 1, p.status, abort_flag);
+                if (!ok) break;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(&kfull[st], S::KV_BYTES);
-                    for (int b = 0; b < QB; ++b)
-                        tma_load_2d(sK + st * S::KV_BYTES + b * BKV * 128, &tmK, &kfull[st], hk * D + b * 64, row);
+                    mbar_arrive_expect_tx(qfull, w.nt * S::Q_BYTES);
+                    for (int t = 0; t < w.nt; ++t)
+                        for (int b = 0; b < QB; ++b)
+                            tma_load_2d(sQ + t * S::Q_BYTES + b * 16384, &tmQ, qfull, w.h * D + b * 64, w.row + 128 * t);
                 }
                 __syncwarp();
-                ki = i + 1;
-                if (!mbar_wait_warp(&vempty[st], ph ^ 1, p.status, abort_flag)) break;
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(&vfull[st], S::KV_BYTES);
-                    for (int b = 0; b < QB; ++b)
-                        tma_load_2d(sV + st * S::KV_BYTES + b * BKV * 128, &tmV, &vfull[st], hk * D + b * 64, row);
+                ++qn;
+                for (int i = 0; i < w.nb; ++i) {
+                    const int st = kn & 1, row = w.k0 + i * BKV;
+                    const uint32_t ph = (kn >> 1) & 1;
+                    ok = mbar_wait_warp(&kempty[st], ph ^ 1, p.status, abort_flag);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(&kfull[st], S::KV_BYTES);
+                        for (int b = 0; b < QB; ++b)
+                            tma_load_2d(sK + st * S::KV_BYTES + b * BKV * 128, &tmK, &kfull[st], hk * D + b * 64, row);
+                    }
+                    __syncwarp();
+                    ++kn;
+                    ok = mbar_wait_warp(&vempty[st], ph ^ 1, p.status, abort_flag);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(&vfull[st], S::KV_BYTES);
+                        for (int b = 0; b < QB; ++b)
+                            tma_load_2d(sV + st * S::KV_BYTES + b * BKV * 128, &tmV, &vfull[st], hk * D + b * 64, row);
+                    }
+                    __syncwarp();
+                    ++vn;
                 }
-                __syncwarp();
-                vi = i + 1;
-            }
-            if (clear && vi == nb) {
-                const int st = (nb - 1) % ST;
-                if (mbar_wait_warp(&vfull[st], ((nb - 1) / ST) & 1, p.status, abort_flag)) {
-                    const int rows = 16 - (tail & 15);
+                if (ok && w.clear) {
+                    const int st = (vn - 1) & 1;
+                    ok = mbar_wait_warp(&vfull[st], ((vn - 1) >> 1) & 1, p.status, abort_flag);
+                    if (!ok) break;
+                    const int rows = 16 - (w.tail & 15);
                     for (int e = lane; e < rows * QB * 8; e += 32) {
-                        const int b = e / (rows * 8), r = tail + e / 8 % rows;
+                        const int b = e / (rows * 8), r = w.tail + e / 8 % rows;
                         *reinterpret_cast<uint4*>(sV + st * S::KV_BYTES + b * BKV * 128 + r * 128 + (e & 7) * 16) =
                             make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(vfixed);
+                    if (lane == 0) mbar_arrive(&vfixed[st]);
                 }
             }
             // every load issued has landed before the CTA may exit
-            mbar_drain(qfull, 0);
-            for (int i = ki > ST ? ki - ST : 0; i < ki; ++i) mbar_drain(&kfull[i % ST], (i / ST) & 1);
-            for (int i = vi > ST ? vi - ST : 0; i < vi; ++i) mbar_drain(&vfull[i % ST], (i / ST) & 1);
-        } else if (warp == 1 && nb > 0) {
+            if (qn > 0) mbar_drain(qfull, (qn - 1) & 1);
+            for (uint32_t i = kn > 2 ? kn - 2 : 0; i < kn; ++i) mbar_drain(&kfull[i & 1], (i >> 1) & 1);
+            for (uint32_t i = vn > 2 ? vn - 2 : 0; i < vn; ++i) mbar_drain(&vfull[i & 1], (i >> 1) & 1);
+        } else if (warp == 1) {
             // ---------------- MMA issuer ----------------
             constexpr uint32_t fmt = F16 ? 0u : 1u;
             constexpr uint32_t idS = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(BKV >> 3) << 17) |
                                      ((uint32_t)(128 >> 4) << 24);
             constexpr uint32_t idO = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
                                      ((uint32_t)(128 >> 4) << 24);
-            const uint64_t qd = sdesc_k128(smem_u32(sQ)), kd = sdesc_k128(smem_u32(sK));
-            const uint64_t vd = sdesc_mn128(smem_u32(sV), BKV * 128);
-            bool issued = false;
-            auto qk = [&](int t, int i) {  // S of block i
-                if (elect_one()) {
-                    const uint32_t d = tmem + S::S_COL(t, i % NS);
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks)
-                        umma_bf16(d, qd + (t * S::Q_BYTES + (ks >> 2) * 16384 + (ks & 3) * 32) / 16,
-                                  kd + (i % ST * S::KV_BYTES + (ks >> 2) * BKV * 128 + (ks & 3) * 32) / 16, idS, ks > 0);
-                    umma_commit(&sfull[t * NS + i % NS]);
-                }
-                __syncwarp();
-                issued = true;
-            };
-            auto pv = [&](int t, int i, bool commit) {  // O += P V of block i
-                const int steps = last_here && i + 1 == nb ? (tail + 15) / 16 : BKV / 16;
-                if (elect_one()) {
-                    const uint32_t d = tmem + S::O_COL(t), a = tmem + S::S_COL(t, i % NS);
-#pragma unroll
-                    for (int kk = 0; kk < BKV / 16; ++kk)
-                        if (kk < steps)
-                            umma_f16_ts(d, a + kk * 8, vd + (i % ST * S::KV_BYTES + kk * 2048) / 16, idO, (i | kk) != 0);
-                    if (commit) umma_commit(&ofull[t]);
-                }
-                __syncwarp();
-            };
-            auto v_ready = [&](int i) -> bool {
-                return mbar_wait_warp(&vfull[i % ST], (i / ST) & 1, p.status, abort_flag) &&
-                       (!clear || i + 1 < nb || mbar_wait_warp(vfixed, 0, p.status, abort_flag));
-            };
+            // The operands of a tcgen05.mma come from uniform registers: stages and
+            // tiles are compile-time constants here, so that descriptors are a
+            // base plus a constant and nothing is moved over for each of them (a
+            // 128 x 128 x 16 product takes the tensor core 64 cycles).
+            const uint32_t qd = static_cast<uint32_t>(sdesc_k128(smem_u32(sQ)));
+            const uint32_t kd = static_cast<uint32_t>(sdesc_k128(smem_u32(sK)));
+            const uint32_t vd = static_cast<uint32_t>(sdesc_mn128(smem_u32(sV), BKV * 128));
+            uint32_t qn = 0, n = 0;             // items and blocks so far
+            uint32_t fixed[2] = {};             // cleared blocks of each stage so far
+            uint32_t cn[NT] = {};               // blocks of each tile so far
+            bool ok = true;
             auto commit_to = [&](uint64_t* bar) {
                 if (elect_one()) umma_commit(bar);
                 __syncwarp();
             };
-            bool ok = mbar_wait_warp(qfull, 0, p.status, abort_flag) &&
-                      mbar_wait_warp(&kfull[0], 0, p.status, abort_flag);
-            if (ok) {
+            auto qk = [&](auto tc, auto stc) {  // S of a block in stage st
+                constexpr int t = decltype(tc)::value, st = decltype(stc)::value;
+                constexpr int buf = NS == 2 ? st : 0;
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks)
+                        umma_f16_ss(tmem + S::S_COL(t, buf), qd + (t * S::Q_BYTES + (ks >> 2) * 16384 + (ks & 3) * 32) / 16,
+                                    kd + (st * S::KV_BYTES + (ks >> 2) * BKV * 128 + (ks & 3) * 32) / 16, idS, ks > 0);
+                    umma_commit(&sfull[t * NS + buf]);
+                }
+                __syncwarp();
+            };
+            // O += P V (O starts as zeros), the steps before the cut as soon as their P is there
+            auto pv = [&](auto tc, auto stc, int steps, bool commit) -> bool {
+                constexpr int t = decltype(tc)::value, st = decltype(stc)::value;
+                constexpr int buf = NS == 2 ? st : 0;
+                const uint32_t ph = cn[t]++ & 1;
+                auto mma = [&](int kk) {
+                    umma_f16_ts(tmem + S::O_COL(t), tmem + S::S_COL(t, buf) + kk * 8, vd + (st * S::KV_BYTES + kk * 2048) / 16,
+                                idO, 1);
+                };
+                if (!mbar_wait_warp(&pfull[2 * t], ph, p.status, abort_flag)) return false;
                 tc_fence_after();
-                for (int t = 0; t < nt; ++t) qk(t, 0);
-                commit_to(&kempty[0]);
-            }
-            for (int i = 0; i < nb && ok; ++i) {
-                const bool more = i + 1 < nb;
-                if (NS == 2 && more) {  // the next block's S runs under this one's softmax
-                    ok = mbar_wait_warp(&kfull[(i + 1) % ST], ((i + 1) / ST) & 1, p.status, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    qk(0, i + 1);
-                    commit_to(&kempty[(i + 1) % ST]);
-                }
-                for (int t = 0; t < nt; ++t) {
-                    ok = mbar_wait_warp(&pfull[t], i & 1, p.status, abort_flag) && (t > 0 || v_ready(i));
-                    if (!ok) break;
-                    tc_fence_after();
-                    pv(t, i, NS == 2 || !more);
-                    if (NS == 1 && more) {
-                        if (t == 0 && !mbar_wait_warp(&kfull[(i + 1) % ST], ((i + 1) / ST) & 1, p.status, abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        qk(t, i + 1);
+                if (elect_one()) {
+                    if (steps >= CUT) {
+#pragma unroll
+                        for (int kk = 0; kk < CUT; ++kk) mma(kk);
+                    } else {
+                        for (int kk = 0; kk < steps; ++kk) mma(kk);
                     }
+                    if (CUT == STEPS && commit) umma_commit(&ofull[t]);
                 }
+                __syncwarp();
+                if constexpr (CUT < STEPS) {
+                    if (!mbar_wait_warp(&pfull[2 * t + 1], ph, p.status, abort_flag)) return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (steps == STEPS) {
+#pragma unroll
+                            for (int kk = CUT; kk < STEPS; ++kk) mma(kk);
+                        } else {
+                            for (int kk = CUT; kk < steps; ++kk) mma(kk);
+                        }
+                        if (commit) umma_commit(&ofull[t]);
+                    }
+                    __syncwarp();
+                }
+                return true;
+            };
+            for (int item = first; item < items && ok; item += stride) {
+                Work w;
+                if (!work_of<D>(p, item, qtiles, rank, split, false, w) || w.nb == 0) continue;
+                // block i of the item, in stage st: its P V, and before (NS == 2) or
+                // between the tiles' (NS == 1) the next block's S
+                auto block = [&](int i, auto stc) -> bool {
+                    constexpr int st = decltype(stc)::value;
+                    constexpr Const<1 - st> next{};
+                    const bool more = i + 1 < w.nb;
+                    const uint32_t ph = (n >> 1) & 1, nph = ((n + 1) >> 1) & 1;
+                    ++n;
+                    const int steps = w.last && !more ? (w.tail + 15) / 16 : STEPS;
+                    if (NS == 2 && more) {
+                        if (!mbar_wait_warp(&kfull[1 - st], nph, p.status, abort_flag)) return false;
+                        tc_fence_after();
+                        qk(Const<0>{}, next);
+                        commit_to(&kempty[1 - st]);
+                        if (i + 2 == w.nb) commit_to(qempty);
+                    }
+                    if (!mbar_wait_warp(&vfull[st], ph, p.status, abort_flag)) return false;
+                    if (w.clear && !more && !mbar_wait_warp(&vfixed[st], fixed[st]++ & 1, p.status, abort_flag))
+                        return false;
+                    if (!pv(Const<0>{}, stc, steps, NS == 2 || !more)) return false;
+                    if (NS == 1 && more) {
+                        if (!mbar_wait_warp(&kfull[1 - st], nph, p.status, abort_flag)) return false;
+                        tc_fence_after();
+                        qk(Const<0>{}, next);
+                    }
+                    if (NT == 2 && w.nt == 2) {
+                        if (!pv(Const<NT - 1>{}, stc, steps, !more)) return false;
+                        if (more) qk(Const<NT - 1>{}, next);
+                    }
+                    commit_to(&vempty[st]);
+                    if (NS == 1 && more) {
+                        commit_to(&kempty[1 - st]);
+                        if (i + 2 == w.nb) commit_to(qempty);
+                    }
+                    return true;
+                };
+                auto begin = [&](auto stc) {
+                    constexpr int st = decltype(stc)::value;
+                    qk(Const<0>{}, stc);
+                    if (NT == 2 && w.nt == 2) qk(Const<NT - 1>{}, stc);
+                    commit_to(&kempty[st]);
+                    if (w.nb == 1) commit_to(qempty);
+                };
+                ok = mbar_wait_warp(qfull, qn++ & 1, p.status, abort_flag) &&
+                     mbar_wait_warp(&kfull[n & 1], (n >> 1) & 1, p.status, abort_flag);
                 if (!ok) break;
-                commit_to(&vempty[i % ST]);
-                if (NS == 1 && more) commit_to(&kempty[(i + 1) % ST]);
+                tc_fence_after();
+                if (n & 1) begin(Const<1>{});
+                else begin(Const<0>{});
+                for (int i = 0; i < w.nb && ok; ++i) ok = n & 1 ? block(i, Const<1>{}) : block(i, Const<0>{});
             }
-            if (issued) {
+            if (qn > 0) {
                 commit_to(drain);
                 mbar_drain(drain, 0);
             }
@@ -285,27 +398,40 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         }
     } else {
         // ---------------- softmax, then the output ----------------
-        float m = -INFINITY, l = 0.f;  // this row's maximum (exp2 domain) and sum
+        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int t = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-        bool done = true;
-        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        if (t < nt) {
-            const float scale = p.scale_log2;
-            const uint32_t tO = tmem + S::O_COL(t) + lane_addr;
-            for (int i = 0; i < nb; ++i) {
-                const uint32_t tS = tmem + S::S_COL(t, i % NS) + lane_addr;
-                done = mbar_wait_warp(&sfull[t * NS + i % NS], (i / NS) & 1, p.status, abort_flag);
+        const uint32_t tO = tmem + S::O_COL(t) + lane_addr;
+        const float scale = p.scale_log2;
+        uint32_t cn = 0, on = 0;        // blocks and outputs of this tile so far
+        float m = -INFINITY, l = 0.f;   // this row's maximum (exp2 domain) and sum
+        Work w;
+        w.nb = 0;
+        bool mine = false, done = true;
+        for (int item = first; item < items && done; item += stride) {
+            mine = work_of<D>(p, item, qtiles, rank, split, false, w) && t < w.nt;
+            if (!mine) continue;
+            m = -INFINITY;
+            l = 0.f;
+            if (w.nb > 0) {
+                const uint32_t zero[16] = {};
+#pragma unroll
+                for (int j = 0; j < D; j += 16) tmem_st16(tO + j, zero);
+            }
+            for (int i = 0; i < w.nb; ++i, ++cn) {
+                const int buf = NS == 2 ? cn & 1 : 0;
+                const uint32_t tS = tmem + S::S_COL(t, buf) + lane_addr;
+                done = mbar_wait_warp(&sfull[t * NS + buf], (cn / NS) & 1, p.status, abort_flag);
                 if (!done) break;
                 tc_fence_after();
                 uint32_t x[BKV];
 #pragma unroll
                 for (int j = 0; j < BKV; j += 32) tmem_ld32(tS + j, *reinterpret_cast<uint32_t(*)[32]>(&x[j]));
                 tmem_ld_wait();
-                if (last_here && i + 1 == nb && tail < BKV) {  // keys past the end
+                if (w.last && i + 1 == w.nb && w.tail < BKV) {  // keys past the end
 #pragma unroll
                     for (int j = 0; j < BKV; ++j)
-                        if (j >= tail) x[j] = 0xff800000u;
+                        if (j >= w.tail) x[j] = 0xff800000u;
                 }
                 float pm[8];
 #pragma unroll
@@ -314,17 +440,17 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 for (int j = 8; j < BKV; j += 2)
                     pm[(j >> 1) & 7] = max3(pm[(j >> 1) & 7], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
                 const float mx =
-                    max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * scale;
+                    max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], pm[7])) * scale;
                 // The maximum in use stays until a block's is more than 8 above it:
                 // P is at most 2^8, O is rescaled rarely, and the division by the sum
-                // cancels it.
+                // cancels it.  A NaN among the scores makes the row one.
                 const float now = mx > m + 8.0f ? mx : m;
-                const float off = now == -INFINITY ? 0.f : -now;
+                const float off = mx != mx ? mx : (now == -INFINITY ? 0.f : -now);
                 const float alpha = exp2_approx(m + off);
                 m = now;
                 if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                     if (NS == 2) {
-                        done = mbar_wait_warp(&ofull[t], (i - 1) & 1, p.status, abort_flag);
+                        done = mbar_wait_warp(&ofull[t], (cn - 1) & 1, p.status, abort_flag);
                         if (!done) break;
                         tc_fence_after();
                     }
@@ -338,107 +464,113 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         tmem_st16(tO + j, o);
                     }
                 }
-                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
+                uint64_t sum2[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < BKV; j += 32) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float a = exp2_approx(fmaf(__uint_as_float(x[j + 2 * e]), scale, off));
-                        const float b = exp2_approx(fmaf(__uint_as_float(x[j + 2 * e + 1]), scale, off));
-                        ls[e & 3] += a + b;
+                        float a, b;
+                        split_pair(fma_pair(pair_of(__uint_as_float(x[j + 2 * e]), __uint_as_float(x[j + 2 * e + 1])), scale2,
+                                            off2), a, b);
+                        a = exp2_approx(a);
+                        b = exp2_approx(b);
+                        sum2[e & 1] = add_pair(sum2[e & 1], pair_of(a, b));
                         // rounded to the 16 bits of V for the product, by at most half a step
                         pk[e] = pack2<F16>(a, b);
                     }
                     tmem_st16(tS + j / 2, pk);
+                    if (j + 32 == S::CUT || j + 32 == BKV) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&pfull[2 * t + (j + 32 > S::CUT)]);
+                    }
                 }
-                l = l * alpha + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[t]);
+                float sa, sb;
+                split_pair(add_pair(sum2[0], sum2[1]), sa, sb);
+                l = l * alpha + (sa + sb);
             }
+            if (!done) break;
             // The last P V.  With two S buffers every P V is a phase of the barrier, and
             // the last S says no more than that the last but two are over: a wait can
             // tell two neighbouring phases apart, not three.
-            if (NS == 2 && nb > 1) done = done && mbar_wait_warp(&ofull[t], nb & 1, p.status, abort_flag);
-            if (nb > 0) done = done && mbar_wait_warp(&ofull[t], NS == 2 ? (nb - 1) & 1 : 0, p.status, abort_flag);
+            if (NS == 2 && w.nb > 1) done = mbar_wait_warp(&ofull[t], cn & 1, p.status, abort_flag);
+            if (w.nb > 0)
+                done = done && mbar_wait_warp(&ofull[t], (NS == 2 ? cn - 1 : on++) & 1, p.status, abort_flag);
+            if (!done) break;
             tc_fence_after();
-        }
-        const int row = q0 + t * 128 + r;
-        const bool stored = t < nt && done && row < c.nq;
-        uint16_t* out = p.out + static_cast<int64_t>(c.q0 + row) * p.ldo + h * D;
-        if (split == 1) {
-            if (t < nt && done) {
+            if (split == 1) {
                 const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
-    #pragma unroll
+                uint16_t* out = p.out + static_cast<int64_t>(w.row + t * 128 + r) * p.ldo + w.h * D;
+#pragma unroll
                 for (int j = 0; j < D; j += 16) {
                     uint32_t o[16];
-                    if (nb > 0) {
-                        tmem_ld16(tmem + S::O_COL(t) + lane_addr + j, o);
+                    if (w.nb > 0) {
+                        tmem_ld16(tO + j, o);
                         tmem_ld_wait();
                     } else {
-    #pragma unroll
+#pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = 0u;
                     }
-                    if (stored) {
-    #pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            uint4 u;
-                            u.x = pack2<F16>(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
-                            u.y = pack2<F16>(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
-                            u.z = pack2<F16>(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
-                            u.w = pack2<F16>(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
-                            *reinterpret_cast<uint4*>(out + j + v * 8) = u;
-                        }
+                    if (t * 128 + r < w.rows) {
+#pragma unroll
+                        for (int v = 0; v < 16; v += 8)
+                            *reinterpret_cast<uint4*>(out + j + v) =
+                                make_uint4(pack2<F16>(__uint_as_float(o[v + 0]) * inv, __uint_as_float(o[v + 1]) * inv),
+                                           pack2<F16>(__uint_as_float(o[v + 2]) * inv, __uint_as_float(o[v + 3]) * inv),
+                                           pack2<F16>(__uint_as_float(o[v + 4]) * inv, __uint_as_float(o[v + 5]) * inv),
+                                           pack2<F16>(__uint_as_float(o[v + 6]) * inv, __uint_as_float(o[v + 7]) * inv));
                     }
                 }
             }
-        } else {
-            // parts [NT][D][128] take the stages' place
+        }
+        if (split > 1) {  // one item: its parts [NT][D][128] take the stages' place
             __syncthreads();
             float* part = reinterpret_cast<float*>(smem);
-            if (t < nt) {
+            if (mine) {
                 sM[t * 128 + r] = m;
                 sL[t * 128 + r] = l;
-    #pragma unroll
+#pragma unroll
                 for (int j = 0; j < D; j += 16) {
                     uint32_t o[16];
-                    if (nb > 0 && done) {
-                        tmem_ld16(tmem + S::O_COL(t) + lane_addr + j, o);
+                    if (w.nb > 0 && done) {
+                        tmem_ld16(tO + j, o);
                         tmem_ld_wait();
                     } else {
-    #pragma unroll
+#pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = 0u;
                     }
-    #pragma unroll
+#pragma unroll
                     for (int e = 0; e < 16; ++e) part[(t * D + j + e) * 128 + r] = __uint_as_float(o[e]);
                 }
             }
             cluster_sync();
-            if (stored) {
+            if (mine && done && t * 128 + r < w.rows) {
                 // this rank's share of the head: columns [rank D / split, (rank + 1) D / split)
-                float w[8], top = -INFINITY, sum = 0.f;
-    #pragma unroll
+                float f[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    w[k] = k < split ? ld_shared_cluster(mapa_shared(smem_u32(sM + t * 128 + r), k)) : -INFINITY;
-                    top = fmaxf(top, w[k]);
+                    f[k] = k < split ? ld_shared_cluster(mapa_shared(smem_u32(sM + t * 128 + r), k)) : -INFINITY;
+                    top = fmaxf(top, f[k]);
                 }
-    #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    w[k] = w[k] == -INFINITY ? 0.f : exp2_approx(w[k] - top);
-                    if (k < split) sum += w[k] * ld_shared_cluster(mapa_shared(smem_u32(sL + t * 128 + r), k));
+                    f[k] = f[k] == -INFINITY ? 0.f : exp2_approx(f[k] - top);
+                    if (k < split) sum += f[k] * ld_shared_cluster(mapa_shared(smem_u32(sL + t * 128 + r), k));
                 }
                 const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+                uint16_t* out = p.out + static_cast<int64_t>(w.row + t * 128 + r) * p.ldo + w.h * D;
                 for (int j = rank * (D / split); j < (rank + 1) * (D / split); j += 8) {
                     float v[8];
-    #pragma unroll
+#pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         v[e] = 0.f;
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            if (k < split && w[k] != 0.f)
-                                v[e] += w[k] * ld_shared_cluster(mapa_shared(smem_u32(part + (t * D + j + e) * 128 + r), k));
+                            if (k < split && f[k] != 0.f)
+                                v[e] += f[k] * ld_shared_cluster(mapa_shared(smem_u32(part + (t * D + j + e) * 128 + r), k));
                         v[e] *= inv;
                     }
                     *reinterpret_cast<uint4*>(out + j) = make_uint4(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]),
@@ -470,14 +602,15 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
         !make_rows_tmap(&tv, p.v, p.f16, p.Tk, static_cast<uint64_t>(p.kv_heads) * D, p.ldv, S::BKV))
         return cudaErrorInvalidValue;
     const int qtiles = (p.max_q + 128 * S::NT - 1) / (128 * S::NT);
-    const int64_t ctas = static_cast<int64_t>(p.nseq) * qtiles * p.heads;
+    const int64_t items = static_cast<int64_t>(p.nseq) * qtiles * p.heads;
+    if (items > 0x7fffffff / 16) return cudaErrorInvalidValue;
     const int blocks = (p.max_kv + S::BKV - 1) / S::BKV;
     // keys are split over up to eight CTAs (of at least eight columns each in
     // the join) while these find room on the SMs and keep two blocks
     int split = 1;
-    while (split < 8 && split * 8 < D && 2 * split * ctas <= num_sms && 4 * split <= blocks) split *= 2;
+    while (split < 8 && split * 8 < D && 2 * split * items <= num_sms && 4 * split <= blocks) split *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.nseq * qtiles * split, p.heads);
+    cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? items * split : std::min<int64_t>(items, num_sms)));
     cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
@@ -490,7 +623,7 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p, split, qtiles);
+    return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p, split, qtiles, static_cast<int>(items));
 }
 
 }  // namespace

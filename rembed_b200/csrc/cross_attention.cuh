@@ -29,13 +29,13 @@ struct CrossParams {
     int* status;
 };
 
-// One query sequence's part, read on the device; false (with kStatusBadShape
-// raised) if it does not lie within the buffers and the given longest lengths.
+// One query sequence's part, read on the device; false (with the status bits
+// `raise`) if it does not lie within the buffers and the given longest lengths.
 struct CrossSeq {
     int q0, nq, k0, nk;
 };
 #ifdef __CUDACC__
-__device__ __forceinline__ bool cross_seq(const CrossParams& p, int s, CrossSeq& c, int bad_shape) {
+__device__ __forceinline__ bool cross_seq(const CrossParams& p, int s, CrossSeq& c, int raise) {
     c.q0 = __ldg(p.cu_q + s);
     const int q1 = __ldg(p.cu_q + s + 1);
     c.k0 = __ldg(p.kv_begin + s);
@@ -43,7 +43,7 @@ __device__ __forceinline__ bool cross_seq(const CrossParams& p, int s, CrossSeq&
     c.nq = q1 - c.q0;
     const bool ok = c.q0 >= 0 && q1 >= c.q0 && q1 <= p.Tq && c.nq <= p.max_q && c.nk >= 0 && c.nk <= p.max_kv &&
                     c.k0 >= 0 && c.k0 <= p.Tk - c.nk;
-    if (!ok && threadIdx.x == 0) atomicOr(p.status, bad_shape);
+    if (!ok && raise) atomicOr(p.status, raise);
     return ok;
 }
 #endif

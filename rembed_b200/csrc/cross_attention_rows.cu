@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
     const int rank = blockIdx.x % split, s = blockIdx.x / split;
     const int hk = blockIdx.y % p.kv_heads, tile = blockIdx.y / p.kv_heads;
     CrossSeq c;
-    if (!cross_seq(p, s, c, kStatusBadShape)) return;  // the same for every CTA of a cluster
+    if (!cross_seq(p, s, c, threadIdx.x == 0 ? kStatusBadShape : 0)) return;  // the same for every CTA of a cluster
     const int rows = min(kRows, c.nq * p.group - tile * kRows);
     if (rows <= 0) return;
 

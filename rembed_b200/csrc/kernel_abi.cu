@@ -356,8 +356,8 @@ int rg_cross_attention(const void* q, const void* k, const void* v, int ldq, int
     const int group = heads / kv_heads;
     max_q = std::min(max_q, Tq);
     max_kv = std::min(max_kv, Tk);
-    // a sequence's grid: at most 8 CTAs for each 16 rows or key/value head, or for each 128 rows
-    if (static_cast<int64_t>(nseq) * ((max_q + 127) / 128) > 0x7fffffff / 8)
+    // tiles of 128 queries of each sequence and head are numbered, with room for a split of each
+    if (static_cast<int64_t>(nseq) * ((max_q + 127) / 128) > 0x7fffffff / 16 / heads)
         return set_err(err, "rg_cross_attention: %d sequences of up to %d queries are too many for one call", nseq, max_q);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
