@@ -28,13 +28,13 @@ constexpr int kRows = 16;
 template <int D>
 struct RowsShape {
     static constexpr int KEYS = D <= 64 ? 32 : 16;  // keys of a chunk
-    static constexpr int STAGES = D == 256 ? 3 : (D == 32 ? 6 : 3);
+    static constexpr int STAGES = D == 32 ? 4 : 2;  // of chunks; three CTAs an SM (head dim 256: one)
     static constexpr int CHUNK = KEYS * D * 2;  // bytes of a chunk of K, and of V
     static constexpr int RING = STAGES * 2 * CHUNK;
     // at the end a warp's 16 x D fp32 outputs take its ring's place
     static_assert(RING >= kRows * D * 4, "a warp's outputs take its ring's place");
-    // ring | m, l [kWarps][kRows] | weights [8 * kWarps][kRows] | 1 / sum [kRows]
-    static constexpr int SMEM = kWarps * RING + (2 * kWarps + 8 * kWarps + 1) * kRows * 4;
+    // rings | maximum, sum, weight [kWarps][kRows] | maximum, sum of all [kRows]
+    static constexpr int SMEM = kWarps * RING + (3 * kWarps + 2) * kRows * 4;
 };
 
 // Byte offset of 16-byte piece c of row r in a chunk, so that eight
@@ -96,8 +96,9 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* sM = reinterpret_cast<float*>(smem + kWarps * S::RING);  // [kWarps][kRows]
     float* sL = sM + kWarps * kRows;
-    float* sW = sL + kWarps * kRows;  // [split * kWarps][kRows]
-    float* sInv = sW + 8 * kWarps * kRows;
+    float* sW = sL + kWarps * kRows;  // [kWarps][kRows]
+    float* sTop = sW + kWarps * kRows;
+    float* sSum = sTop + kRows;
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
 
     // this warp's chunks: step apart from its own number on
@@ -243,43 +244,85 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                 *reinterpret_cast<float2*>(mine + r * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
         }
     }
-    if (split > 1) cluster_sync();
-    else __syncthreads();
-    // the parts' weights: 2^(m - the largest m); the sum of all
-    const int parts = split * kWarps;
+    __syncthreads();
+    // The warps' parts joined: each row's weights 2^(m - the largest m), its sum
+    // and maximum, then its outputs in the first warp's place.
     if (threadIdx.x < rows) {
         const int r = threadIdx.x;
-        float top = -INFINITY, sum = 0.f;
-        for (int i = 0; i < parts; ++i) {
-            const float v = ld_shared_cluster(mapa_shared(smem_u32(sM + (i % kWarps) * kRows + r), split > 1 ? i / kWarps : rank));
-            sW[i * kRows + r] = v;
-            top = fmaxf(top, v);
-        }
-        for (int i = 0; i < parts; ++i) {
-            const float v = sW[i * kRows + r];
-            const float w = v == -INFINITY ? 0.f : ex2(v - top);
+        float top = sM[r], sum = 0.f;
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) top = fmaxf(top, sM[i * kRows + r]);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const float w = sM[i * kRows + r] == -INFINITY ? 0.f : ex2(sM[i * kRows + r] - top);
             sW[i * kRows + r] = w;
-            sum += w * ld_shared_cluster(mapa_shared(smem_u32(sL + (i % kWarps) * kRows + r), split > 1 ? i / kWarps : rank));
+            sum += w * sL[i * kRows + r];
         }
-        sInv[r] = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // no key: zeros; NaN stays
+        sTop[r] = top;
+        sSum[r] = sum;
     }
     __syncthreads();
-    // pairs of neighbouring outputs, shared out over the cluster
-    for (int e = rank * 32 * kWarps + threadIdx.x; e < rows * (D / 2); e += split * 32 * kWarps) {
-        const int r = e / (D / 2), d = (e % (D / 2)) * 2;
-        float a = 0.f, b = 0.f;
-        for (int i = 0; i < parts; ++i) {
+    float* joined = reinterpret_cast<float*>(smem);
+    const float* parts[kWarps];
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) parts[i] = reinterpret_cast<const float*>(smem + i * S::RING);
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * kWarps) {
+        const int r = e / (D / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
             const float w = sW[i * kRows + r];
-            const uint32_t at =
-                mapa_shared(smem_u32(smem + (i % kWarps) * S::RING) + (r * D + d) * 4, split > 1 ? i / kWarps : rank);
+            const float4 f = reinterpret_cast<const float4*>(parts[i])[e];
             if (w != 0.f) {
-                a += w * ld_shared_cluster(at);
-                b += w * ld_shared_cluster(at + 4);
+                v.x = fmaf(w, f.x, v.x);
+                v.y = fmaf(w, f.y, v.y);
+                v.z = fmaf(w, f.z, v.z);
+                v.w = fmaf(w, f.w, v.w);
             }
         }
+        reinterpret_cast<float4*>(joined)[e] = v;
+    }
+    // The same over the CTAs of the cluster, in rank order; the loads of all
+    // ranks are in flight at once.  Each CTA writes its share of the outputs.
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    for (int e = rank * 32 * kWarps + threadIdx.x; e < rows * (D / 2); e += split * 32 * kWarps) {
+        const int r = e / (D / 2), d = (e % (D / 2)) * 2;
+        float a, b, sum;
+        if (split == 1) {
+            a = joined[2 * e];
+            b = joined[2 * e + 1];
+            sum = sSum[r];
+        } else {
+            float w[8], s[8], x[8], y[8], top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t to = k < split ? k : 0;
+                w[k] = ld_shared_cluster(mapa_shared(smem_u32(sTop + r), to));
+                s[k] = ld_shared_cluster(mapa_shared(smem_u32(sSum + r), to));
+                x[k] = ld_shared_cluster(mapa_shared(smem_u32(joined + 2 * e), to));
+                y[k] = ld_shared_cluster(mapa_shared(smem_u32(joined + 2 * e + 1), to));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < split) top = fmaxf(top, w[k]);
+            a = b = sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k >= split || w[k] == -INFINITY) {
+                    if (k < split) sum += 0.f * s[k];  // NaN stays
+                    continue;
+                }
+                const float f = ex2(w[k] - top);
+                sum = fmaf(f, s[k], sum);
+                a = fmaf(f, x[k], a);
+                b = fmaf(f, y[k], b);
+            }
+        }
+        const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // no key: zeros; NaN stays
         const int row = tile * kRows + r;
         uint16_t* out = p.out + static_cast<int64_t>(c.q0 + row / p.group) * p.ldo + (hk * p.group + row % p.group) * D + d;
-        *reinterpret_cast<uint32_t*>(out) = pack2<F16>(a * sInv[r], b * sInv[r]);
+        *reinterpret_cast<uint32_t*>(out) = pack2<F16>(a * inv, b * inv);
     }
     if (split > 1) cluster_sync();  // a CTA's part is read until here
 }

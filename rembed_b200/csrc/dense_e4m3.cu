@@ -232,18 +232,38 @@ __global__ void __launch_bounds__(256, NT == 128 ? 1 : 2)
     const int col = threadIdx.x & 127, n = n0 + col;
     const float b = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
     float amax = 0.f;
-    for (int i = rank * (NT / split) + (threadIdx.x >> 7); i < (rank + 1) * (NT / split); i += 2) {
-        if (m0 + i >= p.M || n >= p.N) break;
-        float v = 0.f;
+    const int i1 = min((rank + 1) * (NT / split), p.M - m0);
+    if (n < p.N) {
         if (split == 1) {
-            v = part[i * 128 + col];
+            for (int i = threadIdx.x >> 7; i < i1; i += 2) {
+                const float v = part[i * 128 + col] + b;
+                store_y<O>(p.y, (m0 + i) * p.ldy + n, v);
+                amax = fmaxf(amax, fabsf(v));
+            }
         } else {
-            const uint32_t at = smem_u32(part + i * 128 + col);
-            for (int r = 0; r < split; ++r) v += ld_shared_cluster(mapa_shared(at, r));
+            // the loads of all ranks, and of two rows, are in flight at once
+            for (int i = rank * (NT / split) + (threadIdx.x >> 7); i < i1; i += 4) {
+                const uint32_t at = smem_u32(part + i * 128 + col), more = i + 2 < i1 ? 2 * 128 * 4 : 0;
+                float f[2][8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const uint32_t to = r < split ? r : 0;
+                    f[0][r] = ld_shared_cluster(mapa_shared(at, to));
+                    f[1][r] = ld_shared_cluster(mapa_shared(at + more, to));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (j == 1 && more == 0) break;
+                    float v = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (r < split) v += f[j][r];
+                    v += b;
+                    store_y<O>(p.y, (m0 + i + 2 * j) * p.ldy + n, v);
+                    amax = fmaxf(amax, fabsf(v));
+                }
+            }
         }
-        v += b;
-        store_y<O>(p.y, (m0 + i) * p.ldy + n, v);
-        amax = fmaxf(amax, fabsf(v));
     }
     if (O == Elem::kF16 && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
     if (split > 1) cluster_sync();  // a CTA's sums are read until here
