@@ -212,61 +212,65 @@ __global__ void __launch_bounds__(256, NT == 128 ? 1 : 2)
         }
         if (!ok) sum[0] = 0.f;  // the status says that the result is not one
     }
-    // every role is done: the stages' memory now holds the sums [NT][128]
+    // Every role of every CTA is done and the stages' memory is free: it takes
+    // the sums, four rows of x to a float4, [split][NT / split / 4][128]: each
+    // CTA's share of the tile's rows from all of them (stores to the owner's
+    // memory, which nothing waits for).
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, S::TMEM_COLS);
     }
-    float* part = reinterpret_cast<float*>(sA);
-    if (warp >= 4) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) part[i * 128 + threadIdx.x - 128] = sum[i];
-    }
-    if (split > 1)
-        cluster_sync();
-    else
-        __syncthreads();
-    // rows [rank NT / split, (rank + 1) NT / split) of the tile, summed over the ranks in order
+    const int lg = __ffs(NT / 4 / split) - 1, per = 1 << lg;  // groups of four rows of a CTA
+    float4* part = reinterpret_cast<float4*>(sA);
     const int col = threadIdx.x & 127, n = n0 + col;
+    if (split > 1) {
+        cluster_sync();
+        if (warp >= 4) {
+            const uint32_t to = smem_u32(part + rank * per * 128 + col);
+#pragma unroll
+            for (int i = 0; i < NT / 4; ++i)
+                if (m0 + 4 * i < p.M)
+                    st_shared_cluster(mapa_shared(to + (i & (per - 1)) * 2048, i >> lg), sum[4 * i], sum[4 * i + 1],
+                                      sum[4 * i + 2], sum[4 * i + 3]);
+        }
+        cluster_sync();
+    } else {
+        if (warp >= 4) {
+#pragma unroll
+            for (int i = 0; i < NT / 4; ++i)
+                part[i * 128 + col] = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+        }
+        __syncthreads();
+    }
     const float b = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
     float amax = 0.f;
-    const int i1 = min((rank + 1) * (NT / split), p.M - m0);
-    if (n < p.N) {
-        if (split == 1) {
-            for (int i = threadIdx.x >> 7; i < i1; i += 2) {
-                const float v = part[i * 128 + col] + b;
-                store_y<O>(p.y, (m0 + i) * p.ldy + n, v);
-                amax = fmaxf(amax, fabsf(v));
+    for (int i = threadIdx.x >> 7; i < per && n < p.N; i += 2) {
+        const int m = m0 + 4 * (rank * per + i);
+        if (m >= p.M) break;
+        float4 f[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < split) f[r] = part[(r * per + i) * 128 + col];
+        float4 v = f[0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r)
+            if (r < split) {
+                v.x += f[r].x;
+                v.y += f[r].y;
+                v.z += f[r].z;
+                v.w += f[r].w;
             }
-        } else {
-            // the loads of all ranks, and of two rows, are in flight at once
-            for (int i = rank * (NT / split) + (threadIdx.x >> 7); i < i1; i += 4) {
-                const uint32_t at = smem_u32(part + i * 128 + col), more = i + 2 < i1 ? 2 * 128 * 4 : 0;
-                float f[2][8];
+        const float out[4] = {v.x + b, v.y + b, v.z + b, v.w + b};
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const uint32_t to = r < split ? r : 0;
-                    f[0][r] = ld_shared_cluster(mapa_shared(at, to));
-                    f[1][r] = ld_shared_cluster(mapa_shared(at + more, to));
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (j == 1 && more == 0) break;
-                    float v = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (r < split) v += f[j][r];
-                    v += b;
-                    store_y<O>(p.y, (m0 + i + 2 * j) * p.ldy + n, v);
-                    amax = fmaxf(amax, fabsf(v));
-                }
+        for (int j = 0; j < 4; ++j)
+            if (m + j < p.M) {
+                store_y<O>(p.y, (m + j) * p.ldy + n, out[j]);
+                amax = fmaxf(amax, fabsf(out[j]));
             }
-        }
     }
     if (O == Elem::kF16 && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
-    if (split > 1) cluster_sync();  // a CTA's sums are read until here
 }
 
 // ---------------------------------------------------------------------------
@@ -640,10 +644,11 @@ cudaError_t launch_thin(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     if (!make_kmajor_tmap(&tw, p.wq, 1, p.N, p.K, p.ldw, 128) || !make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, NT))
         return cudaErrorInvalidValue;
     const int tiles_n = (p.N + 127) / 128, tiles_m = (p.M + NT - 1) / NT, kblocks = (p.K + kE4Block - 1) / kE4Block;
-    // K is split over up to eight CTAs while they find room in one wave
+    // K is split over up to eight CTAs (of at least four rows each in the join)
+    // while they find room in one wave
     const int64_t room = static_cast<int64_t>(num_sms) * (NT == 128 ? 1 : 2);
     int split = 1;
-    while (split < 8 && 2 * split <= kblocks && 2 * split * static_cast<int64_t>(tiles_n) * tiles_m <= room) split *= 2;
+    while (split < 8 && split < NT / 4 && 2 * split <= kblocks && 2 * split * static_cast<int64_t>(tiles_n) * tiles_m <= room) split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles_n * split, tiles_m);
     cfg.blockDim = dim3(S::THREADS);
