@@ -46,7 +46,7 @@ __device__ __forceinline__ void store_y(void* y, int64_t at, float v) {
 template <int NT>
 struct ThinShape {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = NT * 128;
-    static constexpr int STAGES = NT == 128 ? 6 : 4;
+    static constexpr int STAGES = 4;
     static constexpr int ACC = 4;
     static constexpr uint32_t TMEM_COLS = ACC * NT;
     static constexpr int SR = 8;           // ring of scales
@@ -57,7 +57,7 @@ struct ThinShape {
 };
 
 template <int NT, Elem O>
-__global__ void __launch_bounds__(256, NT == 128 ? 1 : 2)
+__global__ void __launch_bounds__(256, 2)
     dense_e4m3_thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                            DenseE4Params p, int split) {
     using S = ThinShape<NT>;
@@ -295,7 +295,7 @@ template <int BN>
 struct WideShape {
     static constexpr int HALF = BN / 2;
     static constexpr int A_BYTES = 128 * 128, B_BYTES = HALF * 128;
-    static constexpr int STAGES = BN == 256 ? 5 : 6;
+    static constexpr int STAGES = BN == 256 ? 5 : 7;
     static constexpr int ACC = 512 / BN;
     static constexpr int WARPS = 8;
     static constexpr int BOXES = 4096;  // a warp's 32 x 32 boxes: one of fp32 or two of 16 bits
@@ -646,7 +646,7 @@ cudaError_t launch_thin(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     const int tiles_n = (p.N + 127) / 128, tiles_m = (p.M + NT - 1) / NT, kblocks = (p.K + kE4Block - 1) / kE4Block;
     // K is split over up to eight CTAs (of at least four rows each in the join)
     // while they find room in one wave
-    const int64_t room = static_cast<int64_t>(num_sms) * (NT == 128 ? 1 : 2);
+    const int64_t room = 2 * static_cast<int64_t>(num_sms);
     int split = 1;
     while (split < 8 && split < NT / 4 && 2 * split <= kblocks && 2 * split * static_cast<int64_t>(tiles_n) * tiles_m <= room) split *= 2;
     cudaLaunchConfig_t cfg = {};
@@ -707,13 +707,21 @@ cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tx, tw, ty, p, tma_out);
 }
 
+// Up to 128 rows the weights' bytes count, and the thin kernel spreads them over
+// the SMs (tiles of 64 rows: 100 x 4096 x 4096 18.4 us against 20.5 for the wide
+// one; 200 x 2048 x 1024 14.3 against 12.3).  Above, the tile width with the
+// cheaper waves: a 128-wide tile takes about 5/8 of a 256-wide one's time
+// (512 x 4096 x 4096: 20.6 against 26.8 us, 1024 x 4096 x 4096: 30.8 against 28.7).
 template <Elem O>
 cudaError_t launch_out(const DenseE4Params& p, int num_sms, cudaStream_t st) {
-    if (p.M > 256) return launch_wide<256, O>(p, num_sms, st);
     if (p.M <= 16) return launch_thin<16, O>(p, num_sms, st);
     if (p.M <= 32) return launch_thin<32, O>(p, num_sms, st);
-    if (p.M <= 64) return launch_thin<64, O>(p, num_sms, st);
-    return launch_thin<128, O>(p, num_sms, st);
+    if (p.M <= 128) return launch_thin<64, O>(p, num_sms, st);
+    const int64_t pairs = num_sms / 2, rows = (p.M + 255) / 256;
+    const int64_t waves256 = (rows * ((p.N + 255) / 256) + pairs - 1) / pairs;
+    const int64_t waves128 = (rows * ((p.N + 127) / 128) + pairs - 1) / pairs;
+    if (5 * waves128 < 8 * waves256) return launch_wide<128, O>(p, num_sms, st);
+    return launch_wide<256, O>(p, num_sms, st);
 }
 
 }  // namespace
