@@ -2,10 +2,16 @@
 // tiles of 128 query rows of one (sequence, query head) against blocks of BKV
 // keys, one pass with the running maximum and sum of the softmax.
 //
-// A CTA stays on its SM and walks items of NT tiles (head dims up to 128: two,
-// 384 threads; 256: one, 256 threads), the next item's loads and first
-// products under the last softmax and the output of the one before.  Roles:
-//   warp 0     TMA producer: the query tiles of an item, K and V blocks through
+// A CTA starts on the item of NT tiles (head dims up to 128: two, 384 threads;
+// 256: one, 256 threads) of its block index and goes on with those of CTAs that
+// have not started yet, taken over through cluster launch control: the next
+// item's loads and first products run under the last softmax and the output of
+// the one before, and the order of the hardware's scheduler evens the load out
+// (8 x 2048 queries over 4096 keys, 12 heads x 64: 305 us in a fixed round of
+// items, 275 in a CTA for each, 262 so).  Roles:
+//   warp 0     takes items over, once the one before is all loaded (taken at its
+//              start they would wait behind it while other SMs idle); TMA
+//              producer of an item's query tiles, and of K and V blocks through
 //              two stages each.  In a text's last block the rows of V behind its
 //              end that share a 16-key MMA step with it are overwritten with
 //              zeros (they may hold anything: 0 * NaN would reach the output);
@@ -23,8 +29,6 @@
 // parts through distributed shared memory in rank order.
 #include <cuda.h>
 #include <cuda_runtime.h>
-
-#include <algorithm>
 
 #include "act16.cuh"
 #include "cross_attention.cuh"
@@ -45,7 +49,7 @@ struct TileShape {
     static constexpr int LOAD = NT * Q_BYTES + 4 * KV_BYTES;  // Q, two stages of K and of V
     static constexpr int PART = NT * D * 512;  // a CTA's fp32 outputs, when keys are split
     static constexpr int RING = LOAD > PART ? LOAD : PART;
-    static constexpr int SMEM = RING + 2 * NT * 512 + 1024 + 256;
+    static constexpr int SMEM = RING + 2 * NT * 512 + 512 + 1024;
     static constexpr uint32_t S_COL(int t, int b) { return (t * NS + b) * BKV; }
     static constexpr uint32_t O_COL(int t) { return NT * NS * BKV + t * D; }
     static constexpr uint32_t TMEM_COLS = NT * NS * BKV + NT * D <= 256 ? 256 : 512;
@@ -132,7 +136,7 @@ __device__ __forceinline__ bool work_of(const CrossParams& p, int item, int qtil
 template <int D, bool F16>
 __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     cross_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, CrossParams p, int split, int qtiles, int items) {
+                       const __grid_constant__ CUtensorMap tmV, CrossParams p, int split, int qtiles) {
     using S = TileShape<D>;
     constexpr int NT = S::NT, NS = S::NS, BKV = S::BKV, QB = S::QB;
     constexpr int STEPS = BKV / 16, CUT = S::CUT / 16;  // MMA steps of a block, and before the cut
@@ -154,12 +158,22 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     uint64_t* pfull = sfull + NT * NS;    // [NT][2]: before and after the cut
     uint64_t* ofull = pfull + NT * 2;     // [NT]
     uint64_t* drain = ofull + NT;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* taken = drain + 1;          // a response has come
+    uint64_t* ifull = taken + 1;          // [2]: an item is there
+    uint64_t* iempty = ifull + 2;         // [2]: every warp has read it
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(iempty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* sItem = reinterpret_cast<int*>(tmem_slot + 2);  // [2]
+    uint8_t* response = smem + S::SMEM - 1024 - 16;
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(qfull, 1);
+        mbar_init(taken, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ifull[i], 1);
+            mbar_init(&iempty[i], 1 + 4 * NT);  // issuer, softmax warps
+        }
         mbar_init(qempty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&kfull[i], 1);
@@ -189,7 +203,16 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     pdl_wait();
     const uint32_t tmem = *tmem_slot;
     const int rank = blockIdx.x % split;
-    const int first = blockIdx.x / split, stride = gridDim.x / split;
+    const int first = blockIdx.x / split;
+    // the item after the k-th of this CTA, -1 when there is none
+    auto next_item = [&](uint32_t k) -> int {
+        if (split > 1) return -1;
+        if (!mbar_wait_warp(&ifull[k & 1], (k >> 1) & 1, p.status, abort_flag)) return -1;
+        const int item = sItem[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&iempty[k & 1]);
+        return item;
+    };
 
     if (warp < 4) {
         if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
@@ -197,7 +220,29 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             // ---------------- TMA producer ----------------
             uint32_t qn = 0, kn = 0, vn = 0;  // items, blocks of K and blocks of V loaded
             bool ok = true;
-            for (int item = first; item < items && ok; item += stride) {
+            // take an item over and pass it on, the k-th
+            auto take = [&](uint32_t k) -> int {
+                if (split > 1 || !mbar_wait_warp(&iempty[k & 1], ((k >> 1) & 1) ^ 1, p.status, abort_flag)) return -1;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(taken, 16);
+                    clc_try_cancel(response, taken);
+                }
+                __syncwarp();
+                if (!mbar_wait_warp(taken, k & 1, p.status, abort_flag)) {
+                    mbar_drain(taken, k & 1);  // the response may still be on its way
+                    return -1;
+                }
+                const int item = clc_taken(response);
+                fence_proxy_async_smem();  // read before the next response is written
+                if (lane == 0) {
+                    sItem[k & 1] = item;
+                    mbar_arrive(&ifull[k & 1]);
+                }
+                __syncwarp();
+                return item;
+            };
+            int item = first;
+            for (uint32_t k = 0; item >= 0 && ok; item = ok ? take(k++) : -1) {
                 Work w;
                 if (!work_of<D>(p, item, qtiles, rank, split, lane == 0, w) || w.nb == 0) continue;
                 const int hk = w.h / p.group;
@@ -323,7 +368,8 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
                 return true;
             };
-            for (int item = first; item < items && ok; item += stride) {
+            int item = first;
+            for (uint32_t k = 0; item >= 0 && ok; item = ok ? next_item(k++) : -1) {
                 Work w;
                 if (!work_of<D>(p, item, qtiles, rank, split, false, w) || w.nb == 0) continue;
                 // block i of the item, in stage st: its P V, and before (NS == 2) or
@@ -408,7 +454,8 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         Work w;
         w.nb = 0;
         bool mine = false, done = true;
-        for (int item = first; item < items && done; item += stride) {
+        int item = first;
+        for (uint32_t k = 0; item >= 0 && done; item = done ? next_item(k++) : -1) {
             mine = work_of<D>(p, item, qtiles, rank, split, false, w) && t < w.nt;
             if (!mine) continue;
             m = -INFINITY;
@@ -610,7 +657,7 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
     int split = 1;
     while (split < 8 && split * 8 < D && 2 * split * items <= num_sms && 4 * split <= blocks) split *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? items * split : std::min<int64_t>(items, num_sms)));
+    cfg.gridDim = dim3(static_cast<unsigned>(items * split));
     cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
@@ -623,7 +670,7 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p, split, qtiles, static_cast<int>(items));
+    return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p, split, qtiles);
 }
 
 }  // namespace

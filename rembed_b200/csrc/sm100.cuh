@@ -161,6 +161,31 @@ __device__ __forceinline__ void prefetch_l2_bulk(const void* gptr, uint32_t byte
                  : "memory");
 }
 
+// ---- cluster launch control ---------------------------------------------------
+// Ask for the block index of a CTA of this grid that has not started yet, which
+// then never will: 16 bytes to `response`, completed on `bar`.
+__device__ __forceinline__ void clc_try_cancel(void* response, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(response)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// blockIdx.x of the CTA a response took, -1 if none was left (no more may be asked for then).
+__device__ __forceinline__ int clc_taken(const void* response) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_u32(response))
+        : "memory");
+    return ok ? static_cast<int>(x) : -1;
+}
+
 // ---- tcgen05 -----------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)),
