@@ -302,7 +302,9 @@ struct WideShape {
     static constexpr int SR = 8;        // ring of scales, 2 x 128 each
     static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + WARPS * BOXES + SR * 1024 + 1024 + 512;
     static constexpr int THREADS = 128 + 32 * WARPS;
-    static constexpr int CONTROL_REGS = 40, SUM_REGS = 232;  // 128 * 40 + 256 * 232 = 384 * 168
+    // 128 * 24 + 256 * 240 = 384 * 168; with 232 for the sums their pairs are
+    // moved about (16384 x 4096 x 4096: 255 against 243 us)
+    static constexpr int CONTROL_REGS = 24, SUM_REGS = 240;
     static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -386,7 +388,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CONTROL_REGS));
         if (warp == 0) {
             int stage = 0;
-            uint32_t phase = 0, issued = 0, parity = 0;
+            uint32_t phase = 0;
+            int issued = 0;  // up to the ring's depth
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
                 const int row = tile / n_tiles * 256 + static_cast<int>(rank) * 128;
@@ -403,8 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                         tma_load_2d_pair(sB + stage * S::B_BYTES, &tmW, full_lead + 8 * stage, kb * 128, col);
                     }
                     __syncwarp();
-                    issued |= 1u << stage;
-                    parity = (parity & ~(1u << stage)) | (phase << stage);
+                    issued = min(issued + 1, STAGES);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1;
@@ -412,12 +414,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                 }
             }
             // the even CTA sees every load of both CTAs land
-            if (rank == 0)
-                for (int s = 0; s < STAGES; ++s)
-                    if (issued & (1u << s)) mbar_drain(&full[s], (parity >> s) & 1);
+            for (; issued > 0; --issued) {
+                if (--stage < 0) {
+                    stage = STAGES - 1;
+                    phase ^= 1;
+                }
+                if (rank == 0) mbar_drain(&full[stage], phase);
+            }
         } else if (warp == 1 && rank == 0) {
             constexpr uint32_t idesc = idesc_e4m3(256, BN);
-            const uint64_t ad0 = sdesc_k128(smem_u32(sA)), bd0 = sdesc_k128(smem_u32(sB));
+            const uint32_t ad0 = static_cast<uint32_t>(sdesc_k128(smem_u32(sA)));
+            const uint32_t bd0 = static_cast<uint32_t>(sdesc_k128(smem_u32(sB)));
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool issued = false, ok = true;
@@ -430,7 +437,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                     }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t ad = ad0 + stage * (S::A_BYTES / 16), bd = bd0 + stage * (S::B_BYTES / 16);
+                        const uint32_t ad = ad0 + stage * (S::A_BYTES / 16), bd = bd0 + stage * (S::B_BYTES / 16);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             umma_f8_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
@@ -524,14 +531,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                 }
                 tc_fence_after();
                 const uint32_t ta = tmem + lane_addr + acc * BN + half * HALF;
-                uint32_t t[2][16];
-                tmem_ld16(ta, t[0]);
+                // 64 columns at a time: the latency of a load from tensor memory, long
+                // while products write there, is met twice instead of eight times
+                constexpr int C = HALF < 64 ? HALF : 64;
+                uint32_t t[C];
 #pragma unroll
-                for (int c = 0; c < HALF / 16; ++c) {
+                for (int c = 0; c < HALF; c += C) {
+#pragma unroll
+                    for (int i = 0; i < C; i += 32) tmem_ld32(ta + c + i, *reinterpret_cast<uint32_t(*)[32]>(&t[i]));
                     tmem_ld_wait();
-                    if (c + 1 < HALF / 16) {
-                        tmem_ld16(ta + (c + 1) * 16, t[(c + 1) & 1]);
-                    } else {  // all of it is in registers: the next MMAs may have the accumulator
+                    if (c + C == HALF) {  // all of it is in registers: the next MMAs may have the accumulator
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -540,10 +549,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        sum[c * 8 + i] =
-                            fma_pair(pair_of(__uint_as_float(t[c & 1][2 * i]), __uint_as_float(t[c & 1][2 * i + 1])), s2,
-                                     sum[c * 8 + i]);
+                    for (int i = 0; i < C / 2; ++i)
+                        sum[c / 2 + i] = fma_pair(pair_of(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), s2,
+                                                  sum[c / 2 + i]);
                 }
                 if (++acc == ACC) {
                     acc = 0;

@@ -399,13 +399,16 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t d_tmem, uint64_t a_desc, u
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+// Descriptors by their low words (umma_f16_ss).
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                              uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "mov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kSdescHigh)
         : "memory");
 }
 // Arrive once on this CTA's mbarrier `bar` when all prior pair MMAs of this
