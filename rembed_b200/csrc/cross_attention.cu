@@ -25,6 +25,9 @@
 // tile of head dim 256 has two S buffers instead.  The tensor core finishes a
 // thread's MMAs in order, so a block's S being ready implies that the tile's
 // earlier P V (two tiles: all of them; one tile: all but the last) are done.
+// A wait tells only two neighbouring phases of its barrier apart, so none may
+// run ahead of its waiter by two: with two S buffers the softmax can be a whole
+// block ahead of the issuer, and P and O have a barrier for each buffer.
 // Few items split the keys over a cluster of up to eight CTAs and join their
 // parts through distributed shared memory in rank order.
 #include <cuda.h>
@@ -56,7 +59,14 @@ struct TileShape {
     static constexpr int THREADS = 128 + 128 * NT;
     // keys whose P is handed over before the rest of their block
     static constexpr int CUT = D == 256 ? BKV : BKV / 2;
+    // Which pair of how many takes its exponentials on the FMA pipe: the
+    // transcendental unit alone needs as long as the tensor core at head dim 128
+    // and twice as long at 64 (8 x 2048 queries over 4096 keys, none, one in
+    // eight, in four, in two: head dim 128 381, 366, 368, 401 us; 64 261, 248,
+    // 246, 272 us).
+    static constexpr int FMA_EVERY = D == 256 ? 64 : (D == 128 ? 8 : 4);
     static_assert(NT * NS * BKV + NT * D <= 512 && SMEM <= 232448, "on-chip memory");
+    static_assert(NS == 1 || (NT == 1 && CUT == BKV), "pfull is by the cut or by the buffer");
 };
 
 template <int N>
@@ -64,8 +74,8 @@ struct Const {
     static constexpr int value = N;
 };
 
-// registers of the two-tile kernel: 128 * 96 + 256 * 200 <= 384 * 168
-constexpr int kControlRegs = 96, kSoftmaxRegs = 200;
+// registers of the two-tile kernel: 128 * 72 + 256 * 216 = 384 * 168
+constexpr int kControlRegs = 72, kSoftmaxRegs = 216;
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -90,6 +100,26 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+// 2^x of a pair on the FMA pipe: n = round(x) by the magic constant 1.5 * 2^23,
+// 2^f on [-1/2, 1/2] by a quartic fitted here for least relative error (2.7e-6
+// in fp32), n added to the exponent.  Clamped at 2^-125, which is nothing beside
+// a sum of at least one; a row with a NaN is one already (below).
+__device__ __forceinline__ void exp2_fma(float& a, float& b) {
+    const uint64_t x = pair_of(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+    const uint64_t magic = pair_of(12582912.0f, 12582912.0f);
+    const uint64_t t = add_pair(x, magic);
+    const uint64_t f = add_pair(x, fma_pair(t, pair_of(-1.0f, -1.0f), magic));
+    uint64_t y = fma_pair(pair_of(0.009570102207362652f, 0.009570102207362652f), f,
+                          pair_of(0.05591785907745361f, 0.05591785907745361f));
+    y = fma_pair(y, f, pair_of(0.240247443318367f, 0.240247443318367f));
+    y = fma_pair(y, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+    y = fma_pair(y, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    float ta, tb;
+    split_pair(y, a, b);
+    split_pair(t, ta, tb);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -155,9 +185,9 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     uint64_t* vempty = vfull + 2;         // [2]
     uint64_t* vfixed = vempty + 2;        // [2]: of a stage, so that none runs ahead of its reader
     uint64_t* sfull = vfixed + 2;         // [NT][NS]
-    uint64_t* pfull = sfull + NT * NS;    // [NT][2]: before and after the cut
-    uint64_t* ofull = pfull + NT * 2;     // [NT]
-    uint64_t* drain = ofull + NT;
+    uint64_t* pfull = sfull + NT * NS;    // [NT][2]: before and after the cut, or of each S buffer
+    uint64_t* ofull = pfull + NT * 2;     // [NT][NS]
+    uint64_t* drain = ofull + NT * NS;
     uint64_t* taken = drain + 1;          // a response has come
     uint64_t* ifull = taken + 1;          // [2]: an item is there
     uint64_t* iempty = ifull + 2;         // [2]: every warp has read it
@@ -184,7 +214,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         }
         for (int i = 0; i < NT * NS; ++i) mbar_init(&sfull[i], 1);
         for (int i = 0; i < NT * 2; ++i) mbar_init(&pfull[i], 4);  // one arrival per softmax warp
-        for (int t = 0; t < NT; ++t) mbar_init(&ofull[t], 1);
+        for (int i = 0; i < NT * NS; ++i) mbar_init(&ofull[i], 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -335,12 +365,12 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             auto pv = [&](auto tc, auto stc, int steps, bool commit) -> bool {
                 constexpr int t = decltype(tc)::value, st = decltype(stc)::value;
                 constexpr int buf = NS == 2 ? st : 0;
-                const uint32_t ph = cn[t]++ & 1;
+                const uint32_t ph = (cn[t]++ / NS) & 1;
                 auto mma = [&](int kk) {
                     umma_f16_ts(tmem + S::O_COL(t), tmem + S::S_COL(t, buf) + kk * 8, vd + (st * S::KV_BYTES + kk * 2048) / 16,
                                 idO, 1);
                 };
-                if (!mbar_wait_warp(&pfull[2 * t], ph, p.status, abort_flag)) return false;
+                if (!mbar_wait_warp(&pfull[2 * t + buf], ph, p.status, abort_flag)) return false;
                 tc_fence_after();
                 if (elect_one()) {
                     if (steps >= CUT) {
@@ -349,7 +379,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     } else {
                         for (int kk = 0; kk < steps; ++kk) mma(kk);
                     }
-                    if (CUT == STEPS && commit) umma_commit(&ofull[t]);
+                    if (CUT == STEPS && commit) umma_commit(&ofull[t * NS + buf]);
                 }
                 __syncwarp();
                 if constexpr (CUT < STEPS) {
@@ -362,7 +392,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         } else {
                             for (int kk = CUT; kk < steps; ++kk) mma(kk);
                         }
-                        if (commit) umma_commit(&ofull[t]);
+                        if (commit) umma_commit(&ofull[t * NS]);
                     }
                     __syncwarp();
                 }
@@ -497,7 +527,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 m = now;
                 if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                     if (NS == 2) {
-                        done = mbar_wait_warp(&ofull[t], (cn - 1) & 1, p.status, abort_flag);
+                        done = mbar_wait_warp(&ofull[t * NS + (cn - 1) % NS], ((cn - 1) / NS) & 1, p.status, abort_flag);
                         if (!done) break;
                         tc_fence_after();
                     }
@@ -521,8 +551,12 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         float a, b;
                         split_pair(fma_pair(pair_of(__uint_as_float(x[j + 2 * e]), __uint_as_float(x[j + 2 * e + 1])), scale2,
                                             off2), a, b);
-                        a = exp2_approx(a);
-                        b = exp2_approx(b);
+                        if (e % S::FMA_EVERY == S::FMA_EVERY - 1) {
+                            exp2_fma(a, b);
+                        } else {
+                            a = exp2_approx(a);
+                            b = exp2_approx(b);
+                        }
                         sum2[e & 1] = add_pair(sum2[e & 1], pair_of(a, b));
                         // rounded to the 16 bits of V for the product, by at most half a step
                         pk[e] = pack2<F16>(a, b);
@@ -532,7 +566,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&pfull[2 * t + (j + 32 > S::CUT)]);
+                        if (lane == 0) mbar_arrive(&pfull[2 * t + (NS == 2 ? buf : j + 32 > S::CUT)]);
                     }
                 }
                 float sa, sb;
@@ -540,12 +574,11 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 l = l * alpha + (sa + sb);
             }
             if (!done) break;
-            // The last P V.  With two S buffers every P V is a phase of the barrier, and
-            // the last S says no more than that the last but two are over: a wait can
-            // tell two neighbouring phases apart, not three.
-            if (NS == 2 && w.nb > 1) done = mbar_wait_warp(&ofull[t], cn & 1, p.status, abort_flag);
-            if (w.nb > 0)
-                done = done && mbar_wait_warp(&ofull[t], (NS == 2 ? cn - 1 : on++) & 1, p.status, abort_flag);
+            // the last P V (one S buffer: only it commits)
+            if (w.nb > 0) {
+                const uint32_t last = NS == 2 ? cn - 1 : on++;
+                done = mbar_wait_warp(&ofull[t * NS + (NS == 2 ? last % NS : 0)], (last / NS) & 1, p.status, abort_flag);
+            }
             if (!done) break;
             tc_fence_after();
             if (split == 1) {

@@ -252,6 +252,31 @@ def test_repeats_in_graphs_and_on_streams(cuda, q, heads, kv_heads, dim):
     one.check()
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("q", [1, 260])
+def test_bits_do_not_depend_on_memory_latency(cuda, heads, kv_heads, dim, q):
+    """The same bits with cold caches, and while copies on another stream hold the loads up: no role of the kernel may
+    run further ahead of another than its barriers can tell."""
+    torch = cuda
+    b = Batch(cuda, [q, q - 1, q, 5], [3000, 130, 1111, 64], heads, kv_heads, dim, "bf16", 21)
+    want = b.run().clone()
+    status(torch)
+    junk = torch.empty((2, 1 << 27), device="cuda", dtype=torch.uint8)
+    side = torch.cuda.Stream()
+    for i in range(12):
+        b.out.fill_(-7.0)
+        junk[0].fill_(i)
+        torch.cuda.synchronize()
+        if i % 2:
+            with torch.cuda.stream(side):
+                for _ in range(4):
+                    junk[1].copy_(junk[0])
+        b.run()
+        status(torch)
+        assert torch.equal(b.out, want)
+    torch.cuda.synchronize()
+
+
 def test_states_to_keys_to_attention(cuda):
     """The operators one after another, as they are used: an encoder's packed float32 states are quantised, projected
     to K and V in 8 bits, and attended to by a prompt, then by single tokens.  The attention is held to its own inputs;
