@@ -131,36 +131,34 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // One item: up to NT tiles of one (sequence, query head), and this CTA's blocks
 // of the sequence's keys.
 struct Work {
-    int h, row, rows;  // query head; first row of q and out; rows from there to the sequence's end
-    int nt;            // tiles with rows
+    int h, row, rows;  // query head, -1 for no more items; first row of q and out; rows from there to the sequence's end
+    int nt;            // tiles with rows, 0 for an item without
     int k0, nb;        // first row of k and v, blocks of keys
-    int tail;          // keys of the text's last block
-    bool last;         // the last of the nb blocks is the text's last
-    bool clear;        // and ends within a 16-key step
+    int tail;          // keys of the last of the nb blocks
+    int clear;         // it ends within a 16-key step
 };
 
 template <int D>
-__device__ __forceinline__ bool work_of(const CrossParams& p, int item, int qtiles, int rank, int split, bool report,
-                                        Work& w) {
+__device__ __forceinline__ Work work_of(const CrossParams& p, int item, int qtiles, int rank, int split, bool report) {
     using S = TileShape<D>;
+    Work w = {};
     const int qt = item % qtiles, sh = item / qtiles;
     w.h = sh % p.heads;
     CrossSeq c;
-    if (!cross_seq(p, sh / p.heads, c, report ? kStatusBadShape : 0)) return false;
+    if (!cross_seq(p, sh / p.heads, c, report ? kStatusBadShape : 0)) return w;
     const int q0 = qt * (128 * S::NT);
     w.row = c.q0 + q0;
     w.rows = c.nq - q0;
-    if (w.rows <= 0) return false;
+    if (w.rows <= 0) return w;
     w.nt = min(S::NT, (w.rows + 127) / 128);
     const int blocks = (c.nk + S::BKV - 1) / S::BKV;
     const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / split);
     const int b1 = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split);
     w.k0 = c.k0 + b0 * S::BKV;
     w.nb = b1 - b0;
-    w.tail = c.nk - (blocks - 1) * S::BKV;
-    w.last = w.nb > 0 && b1 == blocks;
-    w.clear = w.last && (w.tail & 15) != 0;
-    return true;
+    w.tail = b1 == blocks ? c.nk - (blocks - 1) * S::BKV : S::BKV;
+    w.clear = w.nb > 0 && (w.tail & 15) != 0;
+    return w;
 }
 
 template <int D, bool F16>
@@ -193,8 +191,9 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     uint64_t* iempty = ifull + 2;         // [2]: every warp has read it
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(iempty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* sItem = reinterpret_cast<int*>(tmem_slot + 2);  // [2]
+    Work* sWork = reinterpret_cast<Work*>(tmem_slot + 2);  // [2]
     uint8_t* response = smem + S::SMEM - 1024 - 16;
+    static_assert(2 * sizeof(Work) <= 128, "the barriers' 512 bytes");
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -234,14 +233,15 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     const uint32_t tmem = *tmem_slot;
     const int rank = blockIdx.x % split;
     const int first = blockIdx.x / split;
-    // the item after the k-th of this CTA, -1 when there is none
-    auto next_item = [&](uint32_t k) -> int {
-        if (split > 1) return -1;
-        if (!mbar_wait_warp(&ifull[k & 1], (k >> 1) & 1, p.status, abort_flag)) return -1;
-        const int item = sItem[k & 1];
+    // the k-th item of this CTA, as the producer passes it on
+    auto item_at = [&](uint32_t k) -> Work {
+        Work w = {};
+        w.h = -1;
+        if (!mbar_wait_warp(&ifull[k & 1], (k >> 1) & 1, p.status, abort_flag)) return w;
+        w = sWork[k & 1];
         __syncwarp();
         if (lane == 0) mbar_arrive(&iempty[k & 1]);
-        return item;
+        return w;
     };
 
     if (warp < 4) {
@@ -250,9 +250,18 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             // ---------------- TMA producer ----------------
             uint32_t qn = 0, kn = 0, vn = 0;  // items, blocks of K and blocks of V loaded
             bool ok = true;
-            // take an item over and pass it on, the k-th
+            // pass the k-th item on, as others read it from shared memory
+            auto pass = [&](uint32_t k, const Work& w) -> bool {
+                if (!mbar_wait_warp(&iempty[k & 1], ((k >> 1) & 1) ^ 1, p.status, abort_flag)) return false;
+                if (lane == 0) {
+                    sWork[k & 1] = w;
+                    mbar_arrive(&ifull[k & 1]);
+                }
+                __syncwarp();
+                return true;
+            };
+            // take one over: the k-th question; -1 if there is none
             auto take = [&](uint32_t k) -> int {
-                if (split > 1 || !mbar_wait_warp(&iempty[k & 1], ((k >> 1) & 1) ^ 1, p.status, abort_flag)) return -1;
                 if (elect_one()) {
                     mbar_arrive_expect_tx(taken, 16);
                     clc_try_cancel(response, taken);
@@ -264,17 +273,19 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
                 const int item = clc_taken(response);
                 fence_proxy_async_smem();  // read before the next response is written
-                if (lane == 0) {
-                    sItem[k & 1] = item;
-                    mbar_arrive(&ifull[k & 1]);
-                }
-                __syncwarp();
                 return item;
             };
             int item = first;
-            for (uint32_t k = 0; item >= 0 && ok; item = ok ? take(k++) : -1) {
-                Work w;
-                if (!work_of<D>(p, item, qtiles, rank, split, lane == 0, w) || w.nb == 0) continue;
+            for (uint32_t k = 0; ok; ++k) {
+                Work w = {};
+                w.h = -1;
+                if (item >= 0) w = work_of<D>(p, item, qtiles, rank, split, lane == 0);
+                ok = pass(k, w);
+                if (w.h < 0 || !ok) break;
+                if (w.nt == 0 || w.nb == 0) {
+                    item = split > 1 ? -1 : take(k);
+                    continue;
+                }
                 const int hk = w.h / p.group;
                 ok = mbar_wait_warp(qempty, (qn & 1) ^ 1, p.status, abort_flag);
                 if (!ok) break;
@@ -322,6 +333,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&vfixed[st]);
                 }
+                if (ok) item = split > 1 ? -1 : take(k);
             }
             // every load issued has landed before the CTA may exit
             if (qn > 0) mbar_drain(qfull, (qn - 1) & 1);
@@ -398,10 +410,10 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
                 return true;
             };
-            int item = first;
-            for (uint32_t k = 0; item >= 0 && ok; item = ok ? next_item(k++) : -1) {
-                Work w;
-                if (!work_of<D>(p, item, qtiles, rank, split, false, w) || w.nb == 0) continue;
+            for (uint32_t k = 0; ok; ++k) {
+                const Work w = item_at(k);
+                if (w.h < 0) break;
+                if (w.nt == 0 || w.nb == 0) continue;
                 // block i of the item, in stage st: its P V, and before (NS == 2) or
                 // between the tiles' (NS == 1) the next block's S
                 auto block = [&](int i, auto stc) -> bool {
@@ -410,7 +422,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     const bool more = i + 1 < w.nb;
                     const uint32_t ph = (n >> 1) & 1, nph = ((n + 1) >> 1) & 1;
                     ++n;
-                    const int steps = w.last && !more ? (w.tail + 15) / 16 : STEPS;
+                    const int steps = more ? STEPS : (w.tail + 15) / 16;
                     if (NS == 2 && more) {
                         if (!mbar_wait_warp(&kfull[1 - st], nph, p.status, abort_flag)) return false;
                         tc_fence_after();
@@ -479,15 +491,17 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t tO = tmem + S::O_COL(t) + lane_addr;
         const float scale = p.scale_log2;
+        // rows of out on 32-byte boundaries: a thread stores whole sectors
+        const bool sectors = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % 16 == 0;
         uint32_t cn = 0, on = 0;        // blocks and outputs of this tile so far
         float m = -INFINITY, l = 0.f;   // this row's maximum (exp2 domain) and sum
-        Work w;
-        w.nb = 0;
-        bool mine = false, done = true;
-        int item = first;
-        for (uint32_t k = 0; item >= 0 && done; item = done ? next_item(k++) : -1) {
-            mine = work_of<D>(p, item, qtiles, rank, split, false, w) && t < w.nt;
-            if (!mine) continue;
+        Work w = {};  // split: still there for the join
+        bool done = true;
+        for (uint32_t k = 0; done; ++k) {
+            const Work next = item_at(k);
+            if (next.h < 0) break;
+            w = next;
+            if (t >= w.nt) continue;
             m = -INFINITY;
             l = 0.f;
             if (w.nb > 0) {
@@ -505,10 +519,14 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < BKV; j += 32) tmem_ld32(tS + j, *reinterpret_cast<uint32_t(*)[32]>(&x[j]));
                 tmem_ld_wait();
-                if (w.last && i + 1 == w.nb && w.tail < BKV) {  // keys past the end
+                if (i + 1 == w.nb && w.tail < BKV) {  // keys past the end, by chunks
 #pragma unroll
-                    for (int j = 0; j < BKV; ++j)
-                        if (j >= w.tail) x[j] = 0xff800000u;
+                    for (int j = 0; j < BKV; j += 32)
+                        if (j + 32 > w.tail) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (j + e >= w.tail) x[j + e] = 0xff800000u;
+                        }
                 }
                 float pm[8];
 #pragma unroll
@@ -595,13 +613,16 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         for (int e = 0; e < 16; ++e) o[e] = 0u;
                     }
                     if (t * 128 + r < w.rows) {
+                        uint32_t u[8];
 #pragma unroll
-                        for (int v = 0; v < 16; v += 8)
-                            *reinterpret_cast<uint4*>(out + j + v) =
-                                make_uint4(pack2<F16>(__uint_as_float(o[v + 0]) * inv, __uint_as_float(o[v + 1]) * inv),
-                                           pack2<F16>(__uint_as_float(o[v + 2]) * inv, __uint_as_float(o[v + 3]) * inv),
-                                           pack2<F16>(__uint_as_float(o[v + 4]) * inv, __uint_as_float(o[v + 5]) * inv),
-                                           pack2<F16>(__uint_as_float(o[v + 6]) * inv, __uint_as_float(o[v + 7]) * inv));
+                        for (int v = 0; v < 8; ++v)
+                            u[v] = pack2<F16>(__uint_as_float(o[2 * v]) * inv, __uint_as_float(o[2 * v + 1]) * inv);
+                        if (sectors) {
+                            st_global_32(out + j, u);
+                        } else {
+                            *reinterpret_cast<uint4*>(out + j) = make_uint4(u[0], u[1], u[2], u[3]);
+                            *reinterpret_cast<uint4*>(out + j + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+                        }
                     }
                 }
             }
@@ -609,7 +630,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         if (split > 1) {  // one item: its parts [NT][D][128] take the stages' place
             __syncthreads();
             float* part = reinterpret_cast<float*>(smem);
-            if (mine) {
+            if (t < w.nt) {
                 sM[t * 128 + r] = m;
                 sL[t * 128 + r] = l;
 #pragma unroll
@@ -627,7 +648,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
             }
             cluster_sync();
-            if (mine && done && t * 128 + r < w.rows) {
+            if (t < w.nt && done && t * 128 + r < w.rows) {
                 // this rank's share of the head: columns [rank D / split, (rank + 1) D / split)
                 float f[8], top = -INFINITY, sum = 0.f;
 #pragma unroll

@@ -161,6 +161,13 @@ __device__ __forceinline__ void prefetch_l2_bulk(const void* gptr, uint32_t byte
                  : "memory");
 }
 
+// 32 bytes to a 32-byte boundary of global memory: one sector.
+__device__ __forceinline__ void st_global_32(void* to, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // ---- cluster launch control ---------------------------------------------------
 // Ask for the block index of a CTA of this grid that has not started yet, which
 // then never will: 16 bytes to `response`, completed on `bar`.
