@@ -316,7 +316,9 @@ int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, c
  * kv_begin [nseq], kv_len [nseq] are device arrays, read when the call runs;
  * max_q and max_kv bound the lengths they hold and choose the kernel.  A
  * sequence that does not fit the buffers or these bounds is skipped, its output
- * left alone, and rg_kernel_status reports it.  Deterministic. */
+ * left alone, and rg_kernel_status reports it.  Deterministic.  (Like the other
+ * kernel-level calls it takes the device's status word, which the first of them
+ * on a device allocates: make one before a stream capture.) */
 int rg_cross_attention(const void *q, const void *k, const void *v, int ldq, int ldk, int ldv, const int32_t *cu_q,
                        const int32_t *kv_begin, const int32_t *kv_len, int nseq, int Tq, int Tk, int max_q,
                        int max_kv, int heads, int kv_heads, int head_dim, float scale, int dtype, void *out, int ldo,

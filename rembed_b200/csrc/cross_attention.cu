@@ -67,6 +67,12 @@ struct TileShape {
     static constexpr int FMA_EVERY = D == 256 ? 64 : (D == 128 ? 8 : 4);
     static_assert(NT * NS * BKV + NT * D <= 512 && SMEM <= 232448, "on-chip memory");
     static_assert(NS == 1 || (NT == 1 && CUT == BKV), "pfull is by the cut or by the buffer");
+    // The clusters of a split wait for all of their CTAs, and each of these for
+    // its tensor memory.  No other kernel that holds tensor memory while its own
+    // cluster waits may share an SM with one, or two calls on two streams could
+    // wait for each other: two tiles take the SM's registers (384 x 168 of 65536),
+    // one tile its shared memory.
+    static_assert(NT == 2 || SMEM > 160 * 1024, "a CTA has its SM to itself");
 };
 
 template <int N>
@@ -741,9 +747,22 @@ cudaError_t launch_cross_tiles(const CrossParams& p, int head_dim, int num_sms, 
     return cudaErrorInvalidValue;
 }
 
+// The row kernel takes 16 rows of a key/value head to a CTA and reads K and V for
+// each of them, the tile kernel up to 256 rows of a query head.  With every SM
+// busy one tile item costs about as much as the quarters below of row CTAs
+// (64 texts of up to 300 keys, rows against tiles: 12/12 heads x 64 32 tokens 34
+// against 39 us, 48 tokens 45 against 39; 16/8 x 128 16 tokens 41 against 51, 32
+// tokens 63 against 51; 3/1 x 256 8 tokens 19 against 23, 16 tokens 31 against
+// 23); with fewer row CTAs than half the SMs these only gain from more of them
+// (one text of 4096 keys, 8/1 x 128, 24 tokens: 14 against 16 us).
 cudaError_t launch_cross(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st) {
-    const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
-    if (rows <= 64 && (rows + 15) / 16 * p.kv_heads <= 65535) return launch_cross_rows(p, head_dim, num_sms, st);
+    const int quarters = head_dim == 32 ? 12 : (head_dim == 64 ? 8 : (head_dim == 128 ? 6 : 3));
+    const int64_t tiles = (static_cast<int64_t>(p.max_q) * p.group + 15) / 16 * p.kv_heads;
+    const int64_t ctas = p.nseq * tiles;
+    const int64_t tile_rows = head_dim == 256 ? 128 : 256;
+    const int64_t items = p.nseq * ((p.max_q + tile_rows - 1) / tile_rows) * p.heads;
+    if (tiles <= 65535 && (2 * ctas <= num_sms || 4 * ctas <= quarters * items))
+        return launch_cross_rows(p, head_dim, num_sms, st);
     return launch_cross_tiles(p, head_dim, num_sms, st);
 }
 

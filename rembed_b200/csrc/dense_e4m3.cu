@@ -35,8 +35,11 @@ __device__ __forceinline__ void store_y(void* y, int64_t at, float v) {
 // rows (one weight block, so its weight scale is one number per block of K)
 // and NT rows of x, over its share of K; the shares of a cluster's CTAs are
 // joined through distributed shared memory, in rank order.  Such products
-// wait for the weights: at M <= 64 the CTAs of a wave keep two times four
-// stages of 16 KB of them in flight per SM.  Roles (256 threads):
+// wait for the weights: two CTAs an SM keep two times four stages of 16 KB of
+// them in flight (37 x 8192 x 4096: 10.2 us, 34 MB of weights from L2; the first
+// bytes arrive after 1.5 us, the joins take 2.5).  The tensor memory of as many
+// CTAs as shared memory lets on an SM never exceeds it, so none waits for
+// another's.  Roles (256 threads):
 //   warp 0     TMA producer: 128 weight rows and NT x rows of each k-block;
 //   warp 1     MMA issuer, four MMAs per k-block into one of ACC accumulators;
 //   warp 2     TMEM allocator, then the scales of each k-block into a ring in
@@ -54,6 +57,7 @@ struct ThinShape {
     static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + SR * SLOT * 4 + 1024 + 512;
     static constexpr int THREADS = 256;
     static_assert(STAGES * (A_BYTES + B_BYTES) >= NT * 512, "the sums of a CTA take the place of its stages");
+    static_assert(228 * 1024 / SMEM * TMEM_COLS <= 512, "no CTA waits for another's tensor memory");
 };
 
 template <int NT, Elem O>
@@ -276,11 +280,15 @@ __global__ void __launch_bounds__(256, 2)
 // ---------------------------------------------------------------------------
 // Large products: persistent CTA pairs (clusters of 2, cta_group::2) on tiles
 // of 256 x BN.  Per k-block the pair's four MMAs fill one of the TMEM
-// accumulators, and the accumulation must read all of it back: at BN = 256 a
-// CTA's 128 x 256 partial takes the tensor core 512 cycles, its reading (the
-// four sub-partitions together 512 bytes a cycle) and its FMAs (128 a cycle)
-// 256 cycles each, so two accumulators and two warps per sub-partition keep
-// the MMAs fed.  Roles (384 threads):
+// accumulators, which the accumulation warps read back.  At BN = 256 that is 512
+// cycles of the tensor core against 128 x 256 values to read, scale and add per
+// CTA, which bounds the kernel: 16384 x 4096 x 4096 takes 243 us (2265 TFLOP/s;
+// 320 us in a sustained loop, where the card lowers its clock to some 1.45
+// GHz), 162 us with the handshake and the accumulation taken out, 178 without
+// the reading and the additions alone.  What carried it there: MMAs issued from
+// warp-uniform code (elect_one; half the time of a lane's branch), arrivals
+// without release at cluster scope, scales by asynchronous copies, and registers
+// enough for the sums.  Roles (384 threads):
 //   warp 0      TMA producer of its CTA's 128 rows of x and BN / 2 of w;
 //   warp 1      (even CTA) MMA issuer;
 //   warp 2      TMEM allocator;
