@@ -79,19 +79,18 @@ struct Lane {
             }
         }
     }
-    // The V values from column c of a row (`row` its first value); columns
-    // from K on read as zeros.  vec: 16-byte aligned rows.
-    static __device__ __forceinline__ uint4 load(const void* row, int c, int K, bool vec) {
-        if (vec && c + V <= K)
-            return __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + static_cast<int64_t>(c) * BYTES));
+    // Rows aligned to nothing but the element, and the matrix's edges: values l,
+    // l + LANES, ... of the first n of a block (zeros behind them), so that a load
+    // of the lanes is contiguous.
+    static __device__ __forceinline__ uint4 load_strided(const void* block, int l, int n) {
         uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (c + i >= K) break;
+            if (l + i * LANES >= n) continue;
             if constexpr (E == Elem::kF32)
-                w[i] = __ldg(static_cast<const uint32_t*>(row) + c + i);
+                w[i] = __ldg(static_cast<const uint32_t*>(block) + l + i * LANES);
             else
-                w[i >> 1] |= static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(row) + c + i)) << (16 * (i & 1));
+                w[i >> 1] |= static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(block) + l + i * LANES)) << (16 * (i & 1));
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -140,20 +139,21 @@ struct Lane {
         for (int i = 0; i < V / 4; ++i)
             w[i] = to_e4m3x2(f[4 * i], f[4 * i + 1]) | to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16;
     }
-    static __device__ __forceinline__ void store(uint8_t* row, int c, int K, bool vec, const uint4& u, float2 inv) {
-        if (c >= K) return;
+    // A whole block's values as the two loads took them: from column l of it.
+    static __device__ __forceinline__ void store_whole(uint8_t* block, int l, const uint4& u, float2 inv) {
         uint32_t w[V / 4];
         convert(u, inv, w);
-        if (vec && c + V <= K) {
-            if constexpr (V == 8)
-                *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
-            else
-                *reinterpret_cast<uint32_t*>(row + c) = w[0];
-            return;
-        }
+        if constexpr (V == 8)
+            *reinterpret_cast<uint2*>(block + l) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint32_t*>(block + l) = w[0];
+    }
+    static __device__ __forceinline__ void store_strided(uint8_t* block, int l, int n, const uint4& u, float2 inv) {
+        uint32_t w[V / 4];
+        convert(u, inv, w);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (c + i < K) row[c + i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+            if (l + i * LANES < n) block[l + i * LANES] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
     }
 };
 
@@ -182,13 +182,16 @@ template <Elem E>
 constexpr int kGroup = 8 / Lane<E>::ROWS;
 constexpr int kRowWarps = 8;
 
-template <Elem E, bool FULL>
-__device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int64_t first, int b, int lane, bool vec_x,
-                                                    bool vec_q) {
+// How a warp's rows lie: at the edge of the matrix, or whole blocks in rows that
+// are 16-byte aligned or not.
+enum class Part { kEdge, kAligned, kUnaligned };
+
+template <Elem E, Part P>
+__device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int64_t first, int b, int lane) {
     using L = Lane<E>;
-    const int rows = FULL ? 8
+    const int rows = P != Part::kEdge ? 8
                           : static_cast<int>(min(static_cast<int64_t>(8), p.rows - first));
-    const int c = b * kE4Block + (lane % L::LANES) * L::V;
+    const int col0 = b * kE4Block, c = col0 + (lane % L::LANES) * L::V;
     const int mine = lane / L::LANES;  // row of the warp-wide load
     const uint8_t* src = static_cast<const uint8_t*>(p.x) + (first + mine) * p.ldx * L::BYTES;
     uint8_t* dst = p.q + (first + mine) * p.ldq;
@@ -196,11 +199,14 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
     uint4 u[kGroup<E>];
 #pragma unroll
     for (int i = 0; i < kGroup<E>; ++i) {
-        if constexpr (FULL) {
+        if constexpr (P == Part::kAligned) {
             u[i] = __ldg(reinterpret_cast<const uint4*>(src + i * src_step + c * L::BYTES));
+        } else if constexpr (P == Part::kUnaligned) {
+            u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, kE4Block);
         } else {
             u[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (i * L::ROWS + mine < rows) u[i] = L::load(src + i * src_step, c, p.K, vec_x);
+            if (i * L::ROWS + mine < rows)
+                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, p.K - col0);
         }
     }
     // lane `row of the group` takes that row's maximum through the divisions
@@ -225,21 +231,19 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
     for (int i = 0; i < kGroup<E>; ++i) {
         const float2 f = make_float2(__shfl_sync(0xffffffffu, inv.x, i * L::ROWS + mine),
                                      __shfl_sync(0xffffffffu, inv.y, i * L::ROWS + mine));
-        if constexpr (FULL) {
-            uint32_t w[L::V / 4];
-            L::convert(u[i], f, w);
-            if constexpr (L::V == 8)
-                *reinterpret_cast<uint2*>(dst + i * dst_step + c) = make_uint2(w[0], w[1]);
-            else
-                *reinterpret_cast<uint32_t*>(dst + i * dst_step + c) = w[0];
+        if constexpr (P == Part::kAligned) {
+            L::store_whole(dst + i * dst_step, c, u[i], f);
+        } else if constexpr (P == Part::kUnaligned) {
+            L::store_strided(dst + i * dst_step + col0, lane % L::LANES, kE4Block, u[i], f);
         } else {
-            if (i * L::ROWS + mine < rows) L::store(dst + i * dst_step, c, p.K, vec_q, u[i], f);
+            if (i * L::ROWS + mine < rows)
+                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, p.K - col0, u[i], f);
         }
     }
 }
 
 template <Elem E>
-__global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(QuantE4Params p, bool vec_x, bool vec_q) {
+__global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(QuantE4Params p, bool aligned) {
     constexpr int kRowsOf = 8;
     pdl_trigger();
     pdl_wait();
@@ -250,17 +254,19 @@ __global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(Quan
     const int b = static_cast<int>(item - group * kb);
     const int64_t first = group * kRowsOf;
     if (first >= p.rows) return;
-    if (vec_x && vec_q && first + kRowsOf <= p.rows && (b + 1) * kE4Block <= p.K)
-        quantize_rows_group<E, true>(p, first, b, lane, true, true);
+    if (first + kRowsOf > p.rows || (b + 1) * kE4Block > p.K)
+        quantize_rows_group<E, Part::kEdge>(p, first, b, lane);
+    else if (aligned)
+        quantize_rows_group<E, Part::kAligned>(p, first, b, lane);
     else
-        quantize_rows_group<E, false>(p, first, b, lane, vec_x, vec_q);
+        quantize_rows_group<E, Part::kUnaligned>(p, first, b, lane);
 }
 
 // One CTA per 128 x 128 tile, held in registers.
 constexpr int kTileWarps = 16;
 
-template <Elem E, bool FULL>
-__device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t first, int col0, bool vec_x, bool vec_q) {
+template <Elem E, Part P>
+__device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t first, int col0) {
     using L = Lane<E>;
     constexpr int LOADS = kE4Block / (kTileWarps * L::ROWS);
     __shared__ uint32_t part[kTileWarps];
@@ -273,11 +279,14 @@ __device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t fi
     uint4 u[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        if constexpr (FULL) {
+        if constexpr (P == Part::kAligned) {
             u[i] = __ldg(reinterpret_cast<const uint4*>(src + i * src_step + c * L::BYTES));
+        } else if constexpr (P == Part::kUnaligned) {
+            u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, kE4Block);
         } else {
             u[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (r0 + i * kTileWarps * L::ROWS < p.rows) u[i] = L::load(src + i * src_step, c, p.K, vec_x);
+            if (r0 + i * kTileWarps * L::ROWS < p.rows)
+                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, p.K - col0);
         }
     }
     uint32_t m = 0u;
@@ -291,30 +300,30 @@ __device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t fi
     const float s = block_scale(m, inv);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        if constexpr (FULL) {
-            uint32_t w[L::V / 4];
-            L::convert(u[i], inv, w);
-            if constexpr (L::V == 8)
-                *reinterpret_cast<uint2*>(dst + i * dst_step + c) = make_uint2(w[0], w[1]);
-            else
-                *reinterpret_cast<uint32_t*>(dst + i * dst_step + c) = w[0];
+        if constexpr (P == Part::kAligned) {
+            L::store_whole(dst + i * dst_step, c, u[i], inv);
+        } else if constexpr (P == Part::kUnaligned) {
+            L::store_strided(dst + i * dst_step + col0, lane % L::LANES, kE4Block, u[i], inv);
         } else {
-            if (r0 + i * kTileWarps * L::ROWS < p.rows) L::store(dst + i * dst_step, c, p.K, vec_q, u[i], inv);
+            if (r0 + i * kTileWarps * L::ROWS < p.rows)
+                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, p.K - col0, u[i], inv);
         }
     }
     if (threadIdx.x == 0) p.scale[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
 }
 
 template <Elem E>
-__global__ void __launch_bounds__(32 * kTileWarps) quantize_tiles_e4m3_kernel(QuantE4Params p, bool vec_x, bool vec_q) {
+__global__ void __launch_bounds__(32 * kTileWarps) quantize_tiles_e4m3_kernel(QuantE4Params p, bool aligned) {
     pdl_trigger();
     pdl_wait();
     const int64_t first = static_cast<int64_t>(blockIdx.y) * kE4Block;
     const int col0 = blockIdx.x * kE4Block;
-    if (vec_x && vec_q && first + kE4Block <= p.rows && col0 + kE4Block <= p.K)
-        quantize_tile<E, true>(p, first, col0, true, true);
+    if (first + kE4Block > p.rows || col0 + kE4Block > p.K)
+        quantize_tile<E, Part::kEdge>(p, first, col0);
+    else if (aligned)
+        quantize_tile<E, Part::kAligned>(p, first, col0);
     else
-        quantize_tile<E, false>(p, first, col0, vec_x, vec_q);
+        quantize_tile<E, Part::kUnaligned>(p, first, col0);
 }
 
 template <Elem E>
@@ -333,14 +342,14 @@ cudaError_t rows_of(const QuantE4Params& p, cudaStream_t st) {
     const int64_t grid = (warps + kRowWarps - 1) / kRowWarps;
     if (grid > 0x7fffffff) return cudaErrorInvalidValue;
     return launch_pdl(quantize_rows_e4m3_kernel<E>, dim3(static_cast<unsigned>(grid)), dim3(32 * kRowWarps), 0, st, p,
-                      aligned_x<E>(p), aligned_q<E>(p));
+                      aligned_x<E>(p) && aligned_q<E>(p));
 }
 
 template <Elem E>
 cudaError_t tiles_of(const QuantE4Params& p, cudaStream_t st) {
     const dim3 grid((p.K + kE4Block - 1) / kE4Block, (p.rows + kE4Block - 1) / kE4Block);
     if (grid.y > 65535) return cudaErrorInvalidValue;
-    return launch_pdl(quantize_tiles_e4m3_kernel<E>, grid, dim3(32 * kTileWarps), 0, st, p, aligned_x<E>(p), aligned_q<E>(p));
+    return launch_pdl(quantize_tiles_e4m3_kernel<E>, grid, dim3(32 * kTileWarps), 0, st, p, aligned_x<E>(p) && aligned_q<E>(p));
 }
 
 }  // namespace
