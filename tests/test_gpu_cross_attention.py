@@ -156,6 +156,46 @@ def test_keys_split_over_a_cluster(cuda, ql, kl, heads, kv_heads, dim):
     b.check()
 
 
+@pytest.mark.parametrize("q", [1, 300])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_no_text_has_a_key(cuda, q, dim):
+    """Every text empty, max_kv 0: zeros, and rows outside the sequences left alone."""
+    b = Batch(cuda, [q, 0, q], [0, 0, 0], 2, 1, dim, "f16", 31)
+    b.run()
+    status(cuda)
+    b.check()
+
+
+@pytest.mark.parametrize("ql,bound", [([1] * 3000, 1), ([1] * 400, 100), ([130] * 300, 130)])
+def test_many_sequences(cuda, ql, bound):
+    """Thousands of short sequences, and bounds far above the lengths (the kernel is chosen by the bounds)."""
+    kl = [(13 * i) % 40 for i in range(len(ql))]
+    b = Batch(cuda, ql, kl, 2, 2, 32, "bf16", 32)
+    b.max_q, b.max_k = bound, 5000
+    b.run()
+    status(cuda)
+    b.check()
+
+
+def test_beside_a_projection_on_another_stream(cuda):
+    """Calls that split their work over clusters, on two streams at once, leave each other's results alone."""
+    import test_gpu_e4m3 as e4
+
+    torch = cuda
+    b = Batch(cuda, [130], [6000], 2, 2, 64, "bf16", 33)
+    host, ops = e4.operands(torch, 37, 2048, 4096, 34)
+    y = e4.dense(torch, ops, 37, 2048, 4096, None, "bf16")
+    want, ref = b.run().clone(), y.clone()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        b.run(stream=s1.cuda_stream)
+        e4.dense(torch, ops, 37, 2048, 4096, None, "bf16", stream=s2.cuda_stream, y=y)
+    torch.cuda.synchronize()
+    status(torch)
+    assert torch.equal(b.out, want) and torch.equal(y, ref)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
 def test_many_items_of_a_few_blocks(cuda, heads, kv_heads, dim):
     """More (sequence, head, tile) items than SMs, most of one to three key blocks that end inside a 16-key step,
