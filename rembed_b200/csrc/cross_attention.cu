@@ -110,7 +110,7 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 // 2^x of a pair on the FMA pipe: n = round(x) by the magic constant 1.5 * 2^23,
 // 2^f on [-1/2, 1/2] by a quartic fitted here for least relative error (2.7e-6
 // in fp32), n added to the exponent.  Clamped at 2^-125, which is nothing beside
-// a sum of at least one; a row with a NaN is one already (below).
+// a sum of at least one; a row with a NaN or +infinity is NaN already (below).
 __device__ __forceinline__ void exp2_fma(float& a, float& b) {
     const uint64_t x = pair_of(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
     const uint64_t magic = pair_of(12582912.0f, 12582912.0f);
@@ -243,7 +243,9 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
     auto item_at = [&](uint32_t k) -> Work {
         Work w = {};
         w.h = -1;
-        if (!mbar_wait_warp(&ifull[k & 1], (k >> 1) & 1, p.status, abort_flag)) return w;
+        // a warp without rows in an item waits here for as long as the others work
+        // on it; each of their waits has its own limit and ends this one too
+        if (!mbar_wait_warp(&ifull[k & 1], (k >> 1) & 1, p.status, abort_flag, 64 * kWaitLimitCycles)) return w;
         w = sWork[k & 1];
         __syncwarp();
         if (lane == 0) mbar_arrive(&iempty[k & 1]);
@@ -544,9 +546,9 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], pm[7])) * scale;
                 // The maximum in use stays until a block's is more than 8 above it:
                 // P is at most 2^8, O is rescaled rarely, and the division by the sum
-                // cancels it.  A NaN among the scores makes the row one.
+                // cancels it.  A NaN or +infinity among the scores makes the row NaN.
                 const float now = mx > m + 8.0f ? mx : m;
-                const float off = mx != mx ? mx : (now == -INFINITY ? 0.f : -now);
+                const float off = mx < INFINITY ? (now == -INFINITY ? 0.f : -now) : mx - mx;
                 const float alpha = exp2_approx(m + off);
                 m = now;
                 if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {

@@ -93,8 +93,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
 }
 
 // The same by a whole warp, with one answer for all of its lanes.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, volatile int* abort) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort));
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, volatile int* abort,
+                                               long long limit = kWaitLimitCycles) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort, limit));
 }
 
 // Teardown variant: bounded, ignores the abort flag.

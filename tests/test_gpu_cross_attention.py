@@ -248,6 +248,33 @@ def test_infinite_and_nan_values(cuda, q):
     assert bool(torch.isnan(dirty[third, :64]).all()) and torch.equal(dirty[third, 64:128], clean[third, 64:128])
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("q", [3, 150])
+def test_infinite_scores(cuda, heads, kv_heads, dim, q):
+    """An infinity in K at any place of a block: a query that meets it with a positive value is NaN (inf - inf), one
+    with a negative value gives that key no weight."""
+    torch = cuda
+    for key in (0, 1, 5, 6, 7, 14, 15, 31, 40, 63, 64, 127, 130):
+        b = Batch(cuda, [q], [140], heads, kv_heads, dim, "bf16", 40 + key)
+        b.run()
+        keep = [k for k in range(140) if k != key]
+        without = Batch(cuda, [q], [139], heads, kv_heads, dim, "bf16", 1)
+        without.q, without.kv = b.q, b.kv[keep].contiguous()
+        without.out = torch.full_like(b.out, -7.0)
+        without.Tq = b.Tq
+        without.run()
+        without.check()
+        b.kv[key, 0] = float("inf")
+        b.out.fill_(-7.0)
+        got = b.run()[:q, :dim].double()
+        status(torch)
+        up = b.q[:q, 0] > 0
+        assert bool(torch.isnan(got[up]).all())
+        # the same weights from sums in another order: within what both may be off the exact result
+        a, w = got[~up], without.out[:q, :dim].double()[~up]
+        assert a.numel() == 0 or float((a - w).abs().max()) <= 4 * 2.0**-8 * float(b.kv[:, kv_heads * dim:].abs().float().max())
+
+
 @pytest.mark.parametrize("q", [1, 150])
 @pytest.mark.parametrize("table,value,who", [(2, 500, 1), (1, -1, 0), (1, 10**6, 1), (2, -5, 0), (0, -3, 0)])
 def test_bad_tables_are_reported(cuda, q, table, value, who):
