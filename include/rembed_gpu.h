@@ -292,8 +292,9 @@ int rg_quantize_tiles_e4m3(const void *w, int dtype, int ldw, int N, int K, uint
  * ldw (multiples of 16, 16-byte aligned bases; columns from K on are not
  * read), scales as the quantisers write them, bias fp32 or NULL, y [M x N]
  * with row stride ldy in `dtype` (RG_DTYPE_F32, F16 or BF16; columns from N
- * on are left alone).  Any M, N, K >= 1 (M up to 8 388 480).  An fp16 result
- * beyond 65504 raises the overflow status (rg_kernel_status).  Deterministic. */
+ * on are left alone).  Any M, N, K >= 1 (M up to 8 388 480, N and K, as the
+ * quantisers' K, up to 2^31 - 256).  An fp16 result beyond 65504 raises the
+ * overflow status (rg_kernel_status).  Deterministic. */
 int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, const uint8_t *wq, int ldw,
                   const float *w_scale, const float *bias, void *y, int ldy, int dtype, int M, int N, int K,
                   void *stream, char **err);
@@ -311,8 +312,9 @@ int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, c
  *
  * Heads as in rg_attention: query head h at columns h * head_dim, key/value
  * head h / (heads / kv_heads); head dims 32, 64, 128, 256; dtype
- * RG_DTYPE_BF16 or F16 for q, k, v and out; scale positive.  Rows start on
- * 16-byte boundaries (bases, and strides a multiple of 8).  cu_q [nseq + 1],
+ * RG_DTYPE_BF16 or F16 for q, k, v and out; scale in (0, 2e38]; Tq and Tk up to
+ * 2^31 - 256.  Rows start on 16-byte boundaries (bases, and strides a multiple
+ * of 8).  cu_q [nseq + 1],
  * kv_begin [nseq], kv_len [nseq] are device arrays, read when the call runs;
  * max_q and max_kv bound the lengths they hold and choose the kernel.  A
  * sequence that does not fit the buffers or these bounds is skipped, its output

@@ -103,12 +103,16 @@ rg::Elem elem_of(int dtype) {
 }
 
 // The two e4m3 quantisers' common checks; fills p.
+// Row and column numbers of the last, partly filled tile stay within 32 bits.
+constexpr int kMaxExtent = 0x7fffff00;
+
 int quant_e4m3_args(const char* fn, const void* x, int dtype, int ldx, int rows, int K, uint8_t* q, int ldq,
                     float* scale, rg::QuantE4Params* p, char** err) {
     if (!x || !q || !scale) return set_err(err, "%s: null buffer", fn);
     const unsigned size = dtype_size(dtype);
     if (!size) return set_err(err, "%s: unknown dtype %d", fn, dtype);
     if (K <= 0) return set_err(err, "%s: K=%d must be positive", fn, K);
+    if (K > kMaxExtent) return set_err(err, "%s: K=%d is over %d", fn, K, kMaxExtent);
     if (ldx < K || ldq < K) return set_err(err, "%s: a row stride is narrower than K=%d", fn, K);
     if (misaligned(x, size) || misaligned(scale, 4)) return set_err(err, "%s: a buffer is not aligned to its type", fn);
     p->x = x;
@@ -300,6 +304,8 @@ int rg_dense_e4m3(const uint8_t* xq, int ldx, const float* x_scale, int ld_xs, c
     if (misaligned(x_scale, 4) || misaligned(w_scale, 4) || misaligned(bias, 4) || misaligned(y, size))
         return set_err(err, "rg_dense_e4m3: a buffer is not aligned to its type");
     if (M > 65535 * 128) return set_err(err, "rg_dense_e4m3: M=%d is over %d", M, 65535 * 128);
+    if (N > kMaxExtent || K > kMaxExtent)
+        return set_err(err, "rg_dense_e4m3: N=%d or K=%d is over %d", N, K, kMaxExtent);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return set_err(err, "cudaGetDevice: %s", cudaGetErrorString(e));
@@ -352,7 +358,11 @@ int rg_cross_attention(const void* q, const void* k, const void* v, int ldq, int
     if (Tk <= 0 || max_q <= 0 || max_kv < 0)
         return set_err(err, "rg_cross_attention: Tk=%d and max_q=%d must be positive, max_kv=%d not negative", Tk, max_q,
                        max_kv);
-    if (!(scale > 0.f && scale <= 3.0e38f)) return set_err(err, "rg_cross_attention: scale must be positive and finite");
+    if (Tq > kMaxExtent || Tk > kMaxExtent)
+        return set_err(err, "rg_cross_attention: Tq=%d or Tk=%d is over %d", Tq, Tk, kMaxExtent);
+    // the kernels multiply by scale * log2(e), finite too
+    if (!(scale > 0.f && scale <= 2.0e38f))
+        return set_err(err, "rg_cross_attention: scale must be positive and at most 2e38");
     const int group = heads / kv_heads;
     max_q = std::min(max_q, Tq);
     max_kv = std::min(max_kv, Tk);

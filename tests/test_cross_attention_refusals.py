@@ -36,3 +36,12 @@ def test_refuses(change, word):
 def test_no_queries_is_no_work():
     assert call(nseq=0) is None
     assert call(Tq=0) is None
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(scale=2.5e38), "scale"),  # times log2(e) it is infinite in fp32
+    (dict(Tq=0x7fffff01), "over"), (dict(Tk=0x7fffff01), "over"),
+])
+def test_refuses_what_overflows(change, word):
+    msg = call(**change)
+    assert msg and "rg_cross_attention" in msg and word in msg, msg

@@ -79,3 +79,13 @@ def test_reference_product():
     y, scale = ref.dense(xq, xs.T, wq, ws)
     # each factor is off by at most half a step, 2^-4 of its value (or half the smallest step of its block)
     assert np.all(np.abs(y - x.astype(np.float64) @ w.T.astype(np.float64)) <= (2 * 2.0**-4 + 2.0**-7) * scale + 1e-2)
+
+
+def test_refuses_what_overflows():
+    big, ld = 0x7fffff01, 0x7fffff10
+    for name, args in (("rg_quantize_rows_e4m3", {**ROWS, "K": big, "ldx": ld, "ldq": ld}),
+                       ("rg_quantize_tiles_e4m3", {**TILES, "K": big, "ldw": ld, "ldq": ld}),
+                       ("rg_dense_e4m3", {**DENSE, "K": big, "ldx": ld, "ldw": ld}),
+                       ("rg_dense_e4m3", {**DENSE, "N": big, "ldy": ld})):
+        msg = call(name, *args.values())
+        assert msg and name in msg and "over" in msg, msg
