@@ -33,6 +33,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "act16.cuh"
 #include "cross_attention.cuh"
 #include "pdl.cuh"
@@ -694,17 +697,31 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
 }
 
 template <int D, bool F16>
-cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
+CrossPlan plan_tiles(const CrossParams& p, int num_sms) {
+    using S = TileShape<D>;
+    static ClusterCounts known = {};
+    const int qtiles = (p.max_q + 128 * S::NT - 1) / (128 * S::NT);
+    const int blocks = (p.max_kv + S::BKV - 1) / S::BKV;
+    CrossPlan plan = {static_cast<int64_t>(p.nseq) * qtiles * p.heads, 1, cudaSuccess};
+    // keys are split over up to eight CTAs (of at least eight columns each in
+    // the join) while these all run at once and keep two blocks (one text of
+    // 4096 keys, 16/8 heads x 128: 33 us over eight, two rounds of clusters; 28
+    // over four)
+    int fit = 0;
+    plan.error = clusters_at_once(cross_tiles_kernel<D, F16>, S::THREADS, S::SMEM, 1, known, fit);
+    for (int split = 2; split <= 8 && plan.error == cudaSuccess; split *= 2) {
+        if (split * 8 > D || split * plan.ctas > num_sms || 2 * split > blocks) break;
+        plan.error = clusters_at_once(cross_tiles_kernel<D, F16>, S::THREADS, S::SMEM, split, known, fit);
+        if (plan.error != cudaSuccess || plan.ctas > fit) break;
+        plan.split = split;
+    }
+    return plan;
+}
+
+template <int D, bool F16>
+cudaError_t launch_tiles(const CrossParams& p, int split, cudaStream_t st) {
     using S = TileShape<D>;
     auto kern = cross_tiles_kernel<D, F16>;
-    static unsigned configured = 0;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 32 || !(__atomic_load_n(&configured, __ATOMIC_ACQUIRE) & (1u << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (e != cudaSuccess) return e;
-        if (dev < 32) __atomic_fetch_or(&configured, 1u << dev, __ATOMIC_RELEASE);
-    }
     CUtensorMap tq, tk, tv;
     if (!make_rows_tmap(&tq, p.q, p.f16, p.Tq, static_cast<uint64_t>(p.heads) * D, p.ldq, 128) ||
         !make_rows_tmap(&tk, p.k, p.f16, p.Tk, static_cast<uint64_t>(p.kv_heads) * D, p.ldk, S::BKV) ||
@@ -713,11 +730,6 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
     const int qtiles = (p.max_q + 128 * S::NT - 1) / (128 * S::NT);
     const int64_t items = static_cast<int64_t>(p.nseq) * qtiles * p.heads;
     if (items > 0x7fffffff / 16) return cudaErrorInvalidValue;
-    const int blocks = (p.max_kv + S::BKV - 1) / S::BKV;
-    // keys are split over up to eight CTAs (of at least eight columns each in
-    // the join) while these find room on the SMs and keep two blocks
-    int split = 1;
-    while (split < 8 && split * 8 < D && 2 * split * items <= num_sms && 4 * split <= blocks) split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * split));
     cfg.blockDim = dim3(S::THREADS);
@@ -737,10 +749,22 @@ cudaError_t launch_tiles(const CrossParams& p, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_cross_tiles(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st) {
+CrossPlan plan_cross_tiles(const CrossParams& p, int head_dim, int num_sms) {
 #define RG_CROSS_TILES(DD)                                        \
     if (head_dim == DD)                                           \
-        return p.f16 ? launch_tiles<DD, true>(p, num_sms, st) : launch_tiles<DD, false>(p, num_sms, st);
+        return p.f16 ? plan_tiles<DD, true>(p, num_sms) : plan_tiles<DD, false>(p, num_sms);
+    RG_CROSS_TILES(32)
+    RG_CROSS_TILES(64)
+    RG_CROSS_TILES(128)
+    RG_CROSS_TILES(256)
+#undef RG_CROSS_TILES
+    return {0, 1, cudaErrorInvalidValue};
+}
+
+cudaError_t launch_cross_tiles(const CrossParams& p, int head_dim, int split, cudaStream_t st) {
+#define RG_CROSS_TILES(DD)                                        \
+    if (head_dim == DD)                                           \
+        return p.f16 ? launch_tiles<DD, true>(p, split, st) : launch_tiles<DD, false>(p, split, st);
     RG_CROSS_TILES(32)
     RG_CROSS_TILES(64)
     RG_CROSS_TILES(128)
@@ -750,22 +774,39 @@ cudaError_t launch_cross_tiles(const CrossParams& p, int head_dim, int num_sms, 
 }
 
 // The row kernel takes 16 rows of a key/value head to a CTA and reads K and V for
-// each of them, the tile kernel up to 256 rows of a query head.  With every SM
-// busy one tile item costs about as much as the quarters below of row CTAs
-// (64 texts of up to 300 keys, rows against tiles: 12/12 heads x 64 32 tokens 34
-// against 39 us, 48 tokens 45 against 39; 16/8 x 128 16 tokens 41 against 51, 32
-// tokens 63 against 51; 3/1 x 256 8 tokens 19 against 23, 16 tokens 31 against
-// 23); with fewer row CTAs than half the SMs these only gain from more of them
-// (one text of 4096 keys, 8/1 x 128, 24 tokens: 14 against 16 us).
+// each of them, the tile kernel up to 256 rows of a query head.  Each one's time
+// is taken as a start and, for every round of its CTAs over the SMs, a constant
+// and a time for each key that a CTA goes through: microseconds, fitted to calls
+// of 1 to 4 texts of 512 and of 4096 keys with 4 to 256 tokens and to 64 texts
+// of 300 keys (rows against tiles, 2 texts of 4096 keys, 3/1 heads x 256: 32
+// tokens 23 and 25 us, 64 33 and 26, 128 51 and 27; 64 texts, 12/12 x 64: 32
+// tokens 34 and 39 us, 48 45 and 39; 16/8 x 128: 16 tokens 41 and 51, 32 63 and
+// 51).
 cudaError_t launch_cross(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st) {
-    const int quarters = head_dim == 32 ? 12 : (head_dim == 64 ? 8 : (head_dim == 128 ? 6 : 3));
+    struct Cost {
+        float rows, rows_key, start, tiles, tiles_key;
+    };
+    const Cost us = head_dim == 32    ? Cost{1.0f, 0.0050f, 1.2f, 2.0f, 0.0100f}
+                    : head_dim == 64  ? Cost{2.5f, 0.0075f, 5.0f, 2.0f, 0.0100f}
+                    : head_dim == 128 ? Cost{3.5f, 0.0125f, 7.0f, 2.0f, 0.0125f}
+                                      : Cost{5.0f, 0.0172f, 7.0f, 2.0f, 0.0165f};
     const int64_t tiles = (static_cast<int64_t>(p.max_q) * p.group + 15) / 16 * p.kv_heads;
-    const int64_t ctas = p.nseq * tiles;
-    const int64_t tile_rows = head_dim == 256 ? 128 : 256;
-    const int64_t items = p.nseq * ((p.max_q + tile_rows - 1) / tile_rows) * p.heads;
-    if (tiles <= 65535 && (2 * ctas <= num_sms || 4 * ctas <= quarters * items))
-        return launch_cross_rows(p, head_dim, num_sms, st);
-    return launch_cross_tiles(p, head_dim, num_sms, st);
+    const CrossPlan by_tiles = plan_cross_tiles(p, head_dim, num_sms);
+    if (by_tiles.error != cudaSuccess) return by_tiles.error;
+    if (tiles <= 65535) {
+        const CrossPlan by_rows = plan_cross_rows(p, head_dim, num_sms);
+        if (by_rows.error != cudaSuccess) return by_rows.error;
+        auto rounds = [](const CrossPlan& plan, int room) {
+            return std::max(1.0f, static_cast<float>(plan.ctas) * static_cast<float>(plan.split) / static_cast<float>(room));
+        };
+        auto keys = [&](const CrossPlan& plan) { return static_cast<float>(p.max_kv) / static_cast<float>(plan.split); };
+        // at head dim 256 an SM holds one row CTA: a started round takes as long as a full one
+        const float turns = head_dim == 256 ? std::ceil(rounds(by_rows, num_sms)) : rounds(by_rows, 2 * num_sms);
+        const float rows = turns * (us.rows + us.rows_key * keys(by_rows));
+        const float whole = us.start + rounds(by_tiles, num_sms) * (us.tiles + us.tiles_key * keys(by_tiles));
+        if (rows <= whole) return launch_cross_rows(p, head_dim, by_rows.split, st);
+    }
+    return launch_cross_tiles(p, head_dim, by_tiles.split, st);
 }
 
 }  // namespace rg

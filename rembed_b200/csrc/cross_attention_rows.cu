@@ -328,25 +328,31 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
 }
 
 template <int D, bool F16>
-cudaError_t launch_rows(const CrossParams& p, int num_sms, cudaStream_t st) {
+CrossPlan plan_rows(const CrossParams& p, int num_sms) {
     using S = RowsShape<D>;
-    auto kern = cross_rows_kernel<D, F16>;
-    static unsigned configured = 0;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 32 || !(__atomic_load_n(&configured, __ATOMIC_ACQUIRE) & (1u << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (e != cudaSuccess) return e;
-        if (dev < 32) __atomic_fetch_or(&configured, 1u << dev, __ATOMIC_RELEASE);
-    }
-    const int tiles = (p.max_q * p.group + kRows - 1) / kRows;
+    static ClusterCounts known = {};
+    const int64_t tiles = (static_cast<int64_t>(p.max_q) * p.group + kRows - 1) / kRows;
     const int chunks = (p.max_kv + S::KEYS - 1) / S::KEYS;
+    CrossPlan plan = {p.nseq * p.kv_heads * tiles, 1, cudaSuccess};
     // the keys are split over up to eight CTAs while these find room on the SMs
     // and each warp keeps a few chunks
-    const int64_t ctas = static_cast<int64_t>(p.nseq) * p.kv_heads * tiles;
     const int64_t room = static_cast<int64_t>(num_sms) * (D == 256 ? 1 : 2);
-    int split = 1;
-    while (split < 8 && 2 * split * ctas <= room && 2 * split * kWarps * 2 <= chunks) split *= 2;
+    int fit = 0;
+    plan.error = clusters_at_once(cross_rows_kernel<D, F16>, 32 * kWarps, S::SMEM, 1, known, fit);
+    for (int split = 2; split <= 8 && plan.error == cudaSuccess; split *= 2) {
+        if (split * plan.ctas > room || split * kWarps * 2 > chunks) break;
+        plan.error = clusters_at_once(cross_rows_kernel<D, F16>, 32 * kWarps, S::SMEM, split, known, fit);
+        if (plan.error != cudaSuccess || plan.ctas > fit) break;
+        plan.split = split;
+    }
+    return plan;
+}
+
+template <int D, bool F16>
+cudaError_t launch_rows(const CrossParams& p, int split, cudaStream_t st) {
+    using S = RowsShape<D>;
+    auto kern = cross_rows_kernel<D, F16>;
+    const int tiles = (p.max_q * p.group + kRows - 1) / kRows;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.nseq * split, p.kv_heads * tiles);
     cfg.blockDim = dim3(32 * kWarps);
@@ -366,10 +372,22 @@ cudaError_t launch_rows(const CrossParams& p, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_cross_rows(const CrossParams& p, int head_dim, int num_sms, cudaStream_t st) {
+CrossPlan plan_cross_rows(const CrossParams& p, int head_dim, int num_sms) {
 #define RG_CROSS_ROWS(DD)                                         \
     if (head_dim == DD)                                           \
-        return p.f16 ? launch_rows<DD, true>(p, num_sms, st) : launch_rows<DD, false>(p, num_sms, st);
+        return p.f16 ? plan_rows<DD, true>(p, num_sms) : plan_rows<DD, false>(p, num_sms);
+    RG_CROSS_ROWS(32)
+    RG_CROSS_ROWS(64)
+    RG_CROSS_ROWS(128)
+    RG_CROSS_ROWS(256)
+#undef RG_CROSS_ROWS
+    return {0, 1, cudaErrorInvalidValue};
+}
+
+cudaError_t launch_cross_rows(const CrossParams& p, int head_dim, int split, cudaStream_t st) {
+#define RG_CROSS_ROWS(DD)                                         \
+    if (head_dim == DD)                                           \
+        return p.f16 ? launch_rows<DD, true>(p, split, st) : launch_rows<DD, false>(p, split, st);
     RG_CROSS_ROWS(32)
     RG_CROSS_ROWS(64)
     RG_CROSS_ROWS(128)

@@ -375,3 +375,49 @@ def test_states_to_keys_to_attention(cuda):
     exact = states.double() @ w.double().t()
     rel = float((b.kv.double() - exact).norm() / exact.norm())
     assert rel <= math.sqrt(2) * 2.0**-3 / math.sqrt(12) + 2.0**-8
+
+
+FIRST_IN_GRAPH = """
+import ctypes, sys
+sys.path[:0] = {paths!r}
+import torch
+import test_gpu_cross_attention as t
+from rembed_b200.embedder import library
+err = ctypes.c_char_p()
+assert library().rg_kernel_status(None, ctypes.byref(err)) == 0
+calls = [t.Batch(torch, q, [700, 2000], heads, kv_heads, dim, "bf16", 5)
+         for q, heads, kv_heads, dim in (([1, 1], 4, 2, 64), ([300, 200], 4, 2, 128), ([150, 3], 3, 1, 256))]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    for c in calls:
+        c.run()
+g.replay()
+t.status(torch)
+for c in calls:
+    c.check()
+"""
+
+
+def test_first_calls_in_a_capture(cuda):
+    """Once the device has its status word, a kernel's first call may be one that is captured."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_GRAPH.format(paths=[os.path.dirname(here), here])], timeout=300,
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("nseq,q,keys,heads,kv_heads,dim", [
+    (2, 40, 4096, 3, 1, 256), (2, 128, 4096, 3, 1, 256), (1, 96, 4096, 3, 1, 256), (2, 200, 4096, 8, 1, 128),
+    (1, 200, 4096, 16, 8, 128), (4, 64, 4096, 12, 12, 64), (1, 64, 2048, 12, 12, 64), (2, 64, 4096, 12, 12, 32),
+])
+def test_few_long_texts(cuda, nseq, q, keys, heads, kv_heads, dim):
+    """Keys split over clusters of every size, as the SMs have room for them, by the rows' kernel and by the tiles'."""
+    one = Batch(cuda, [q - s for s in range(nseq)], [keys - 100 * s for s in range(nseq)], heads, kv_heads, dim, "bf16", 21)
+    one.run()
+    status(cuda)
+    one.check()
