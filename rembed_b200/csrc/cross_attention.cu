@@ -37,6 +37,7 @@
 #include <cmath>
 
 #include "act16.cuh"
+#include "clusters.cuh"
 #include "cross_attention.cuh"
 #include "pdl.cuh"
 #include "sm100.cuh"

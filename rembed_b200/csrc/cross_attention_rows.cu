@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include "act16.cuh"
+#include "clusters.cuh"
 #include "cross_attention.cuh"
 #include "pdl.cuh"
 #include "sm100.cuh"

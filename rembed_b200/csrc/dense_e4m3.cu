@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "act16.cuh"
 #include "e4m3.cuh"
 #include "gemm.cuh"
@@ -649,8 +651,21 @@ cudaError_t allow_smem(K kern, int bytes, unsigned& configured) {
     return e;
 }
 
+// K is split over up to eight CTAs (of at least four rows each in the join)
+// while they all run at once: two an SM, of which clusters of four and eight
+// leave a tenth empty, as they do not cross GPCs (256 of them ran at once; of 288
+// and 296 some waited: 100 x 4736 x 16384 47 us over four, 39 over two).
+int thin_split(const DenseE4Params& p, int nt, int num_sms) {
+    const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + nt - 1) / nt);
+    const int kblocks = (p.K + kE4Block - 1) / kE4Block;
+    int split = 1;
+    for (int s = 2; s <= 8 && s <= nt / 4 && s <= kblocks; s *= 2)
+        if (s * tiles <= (s == 2 ? 2 * num_sms : 2 * num_sms * 9 / 10)) split = s;
+    return split;
+}
+
 template <int NT, Elem O>
-cudaError_t launch_thin(const DenseE4Params& p, int num_sms, cudaStream_t st) {
+cudaError_t launch_thin(const DenseE4Params& p, int split, cudaStream_t st) {
     using S = ThinShape<NT>;
     static unsigned configured = 0;
     auto kern = dense_e4m3_thin_kernel<NT, O>;
@@ -659,12 +674,7 @@ cudaError_t launch_thin(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     CUtensorMap tw, tx;
     if (!make_kmajor_tmap(&tw, p.wq, 1, p.N, p.K, p.ldw, 128) || !make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, NT))
         return cudaErrorInvalidValue;
-    const int tiles_n = (p.N + 127) / 128, tiles_m = (p.M + NT - 1) / NT, kblocks = (p.K + kE4Block - 1) / kE4Block;
-    // K is split over up to eight CTAs (of at least four rows each in the join)
-    // while they find room in one wave
-    const int64_t room = 2 * static_cast<int64_t>(num_sms);
-    int split = 1;
-    while (split < 8 && split < NT / 4 && 2 * split <= kblocks && 2 * split * static_cast<int64_t>(tiles_n) * tiles_m <= room) split *= 2;
+    const int tiles_n = (p.N + 127) / 128, tiles_m = (p.M + NT - 1) / NT;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles_n * split, tiles_m);
     cfg.blockDim = dim3(S::THREADS);
@@ -723,20 +733,33 @@ cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tx, tw, ty, p, tma_out);
 }
 
-// Up to 128 rows the weights' bytes count, and the thin kernel spreads them over
-// the SMs (tiles of 64 rows: 100 x 4096 x 4096 18.4 us against 20.5 for the wide
-// one; 200 x 2048 x 1024 14.3 against 12.3).  Above, the tile width with the
-// cheaper waves: a 128-wide tile takes about 5/8 of a 256-wide one's time
-// (512 x 4096 x 4096: 20.6 against 26.8 us, 1024 x 4096 x 4096: 30.8 against 28.7).
+// Up to 32 rows the weights' bytes count, and the thin kernel spreads them over
+// the SMs.  Above, the kernel and tile width whose waves are estimated to take
+// less, in microseconds a k-block: a pair's tile of 256 columns 0.50, of 128
+// 0.33; thin tiles of 64 rows 0.5 while each has an SM to itself, two an SM
+// 0.75, and 3 for their start and join (thin against wide: 100 x 4096 x 4096
+// 16 and 18.5 us, 100 x 16384 x 16384 90 and 76, 200 x 1024 x 16384 22 and 45,
+// 200 x 4096 x 4096 22.5 and 18.5, 300 x 1024 x 4096 16 and 18.5; widths 128 and
+// 256: 512 x 4096 x 4096 21 and 27, 1024 x 4096 x 4096 31 and 29).
 template <Elem O>
 cudaError_t launch_out(const DenseE4Params& p, int num_sms, cudaStream_t st) {
-    if (p.M <= 16) return launch_thin<16, O>(p, num_sms, st);
-    if (p.M <= 32) return launch_thin<32, O>(p, num_sms, st);
-    if (p.M <= 128) return launch_thin<64, O>(p, num_sms, st);
+    if (p.M <= 16) return launch_thin<16, O>(p, thin_split(p, 16, num_sms), st);
+    if (p.M <= 32) return launch_thin<32, O>(p, thin_split(p, 32, num_sms), st);
+    const int64_t kblocks = (p.K + kE4Block - 1) / kE4Block;
     const int64_t pairs = num_sms / 2, rows = (p.M + 255) / 256;
     const int64_t waves256 = (rows * ((p.N + 255) / 256) + pairs - 1) / pairs;
     const int64_t waves128 = (rows * ((p.N + 127) / 128) + pairs - 1) / pairs;
-    if (5 * waves128 < 8 * waves256) return launch_wide<128, O>(p, num_sms, st);
+    const float wide256 = 0.50f * static_cast<float>(waves256), wide128 = 0.33f * static_cast<float>(waves128);
+    const int64_t tiles_m = (p.M + 63) / 64;
+    if (tiles_m <= 65535) {
+        const int split = thin_split(p, 64, num_sms);
+        const int64_t ctas = tiles_m * ((p.N + 127) / 128) * split;
+        const int64_t waves = (ctas + 2 * num_sms - 1) / (2 * num_sms);
+        const float block = ctas <= num_sms ? 0.5f : 0.75f * static_cast<float>(waves);
+        const float thin = 3.0f + block * static_cast<float>((kblocks + split - 1) / split);
+        if (thin <= std::min(wide256, wide128) * static_cast<float>(kblocks)) return launch_thin<64, O>(p, split, st);
+    }
+    if (wide128 < wide256) return launch_wide<128, O>(p, num_sms, st);
     return launch_wide<256, O>(p, num_sms, st);
 }
 

@@ -256,3 +256,19 @@ def test_quantise_then_project(cuda):
     rel = float((y.double() - want).norm() / want.norm())
     # independent errors: each factor's relative error is uniform within a step of 2^-3 to 2^-4 of it, rms below 2^-3 / sqrt(12)
     assert rel <= math.sqrt(2) * 2.0**-3 / math.sqrt(12)
+
+
+@pytest.mark.parametrize("M,N,K", [
+    (200, 130, 2048), (300, 100, 2100), (520, 64, 4000), (129, 257, 1500), (1000, 128, 3000),  # few columns, long K
+    (70, 9500, 260), (33, 9500, 384), (128, 10001, 129),  # few rows, many columns
+    (64, 4736, 1300), (100, 4736, 1100), (40, 2300, 2050),  # as many clusters as SMs have room for, or more
+])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_dense_where_the_kernels_meet(cuda, M, N, K, dtype):
+    """Few rows through the pairs' kernel, more of them through the one that splits K."""
+    torch = cuda
+    host, ops = operands(torch, M, N, K, M + N + K)
+    bias = torch.randn((N,), device="cuda")
+    y = dense(torch, ops, M, N, K, bias, dtype)
+    status(torch)
+    check(torch, y, host, bias, dtype, M, N, K, N, 0)
