@@ -191,7 +191,9 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
     using L = Lane<E>;
     const int rows = P != Part::kEdge ? 8
                           : static_cast<int>(min(static_cast<int64_t>(8), p.rows - first));
-    const int col0 = b * kE4Block, c = col0 + (lane % L::LANES) * L::V;
+    // a row may be wider than 2^31 bytes
+    const int64_t col0 = static_cast<int64_t>(b) * kE4Block, c = col0 + (lane % L::LANES) * L::V;
+    const int behind = static_cast<int>(min(static_cast<int64_t>(kE4Block), p.K - col0));  // columns from col0 on
     const int mine = lane / L::LANES;  // row of the warp-wide load
     const uint8_t* src = static_cast<const uint8_t*>(p.x) + (first + mine) * p.ldx * L::BYTES;
     uint8_t* dst = p.q + (first + mine) * p.ldq;
@@ -206,7 +208,7 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
         } else {
             u[i] = make_uint4(0u, 0u, 0u, 0u);
             if (i * L::ROWS + mine < rows)
-                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, p.K - col0);
+                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, behind);
         }
     }
     // lane `row of the group` takes that row's maximum through the divisions
@@ -237,7 +239,7 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
             L::store_strided(dst + i * dst_step + col0, lane % L::LANES, kE4Block, u[i], f);
         } else {
             if (i * L::ROWS + mine < rows)
-                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, p.K - col0, u[i], f);
+                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, behind, u[i], f);
         }
     }
 }
@@ -266,12 +268,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_e4m3_kernel(Quan
 constexpr int kTileWarps = 16;
 
 template <Elem E, Part P>
-__device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t first, int col0) {
+__device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t first, int64_t col0) {
     using L = Lane<E>;
     constexpr int LOADS = kE4Block / (kTileWarps * L::ROWS);
     __shared__ uint32_t part[kTileWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = col0 + (lane % L::LANES) * L::V;
+    const int64_t c = col0 + (lane % L::LANES) * L::V;  // a row may be wider than 2^31 bytes
+    const int behind = static_cast<int>(min(static_cast<int64_t>(kE4Block), p.K - col0));  // columns from col0 on
     const int64_t r0 = first + warp * L::ROWS + lane / L::LANES;
     const uint8_t* src = static_cast<const uint8_t*>(p.x) + r0 * p.ldx * L::BYTES;
     uint8_t* dst = p.q + r0 * p.ldq;
@@ -286,7 +289,7 @@ __device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t fi
         } else {
             u[i] = make_uint4(0u, 0u, 0u, 0u);
             if (r0 + i * kTileWarps * L::ROWS < p.rows)
-                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, p.K - col0);
+                u[i] = L::load_strided(src + i * src_step + col0 * L::BYTES, lane % L::LANES, behind);
         }
     }
     uint32_t m = 0u;
@@ -306,7 +309,7 @@ __device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t fi
             L::store_strided(dst + i * dst_step + col0, lane % L::LANES, kE4Block, u[i], inv);
         } else {
             if (r0 + i * kTileWarps * L::ROWS < p.rows)
-                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, p.K - col0, u[i], inv);
+                L::store_strided(dst + i * dst_step + col0, lane % L::LANES, behind, u[i], inv);
         }
     }
     if (threadIdx.x == 0) p.scale[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(32 * kTileWarps) quantize_tiles_e4m3_kernel(Qu
     pdl_trigger();
     pdl_wait();
     const int64_t first = static_cast<int64_t>(blockIdx.y) * kE4Block;
-    const int col0 = blockIdx.x * kE4Block;
+    const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kE4Block;
     if (first + kE4Block > p.rows || col0 + kE4Block > p.K)
         quantize_tile<E, Part::kEdge>(p, first, col0);
     else if (aligned)
