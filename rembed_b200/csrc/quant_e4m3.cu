@@ -7,16 +7,15 @@
 // (next to x / 2^-126 where the scale is that).  The quotient is rounded once,
 // from its exact value: a product with a rounded reciprocal would put values
 // on the wrong side of a tie, and with 16-bit inputs exact ties are common.
-// With r + d = 448 / a (r the quotient towards zero, d its remainder's, both
-// once per block) and y = x r rounded, y + ((x r - y) + x d) is the quotient to
-// some 2^-47 of itself.  16-bit x and a cannot come nearer to a tie than 2^-18
-// without being one, so there its nearest float says all.  For fp32 the
-// products with r (1 -+ 2^-22) enclose it, and where both round to the same
-// bytes that is the answer; else the sum is cut to a float whose last bit is
-// set if anything was cut off, which four bits' rounding cannot mistake for a
-// tie.
+// 16-bit x and a cannot come nearer to a tie than 2^-18 without being one: with
+// r + d = 448 / a (r the quotient towards zero, d its remainder's, both once per
+// block) and y = x r rounded, y + ((x r - y) + x d) is the quotient to some 2^-30
+// of itself or better, and its nearest float says all.  fp32 can come as near as
+// 2^-30: the products with r (1 -+ 2^-21) enclose the quotient, and where they
+// round to different bytes the value is compared with the midpoint t between the
+// two, 448 x with t a, both as exact sums of two floats.
 // A NaN in a block makes the scale NaN, an infinity makes it infinite (with
-// r = d = 0: the infinity becomes NaN, the others 0, and 0 * inf is NaN): a
+// r = 0: the infinity becomes NaN, the others 0, and 0 * inf is NaN): a
 // block that held either is NaN all over once it is scaled back.
 //
 // Both kernels are bound by HBM: each value is read once into registers, the
@@ -41,14 +40,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // x (r + d) rounded so that its rounding to e4m3 is that of the exact product.
 __device__ __forceinline__ float scaled16(float x, float2 inv) {
-    const float y = x * inv.x;
-    return y + __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y));
+    const float y = __fmul_rn(x, inv.x);
+    return __fadd_rn(y, __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y)));
 }
-__device__ __forceinline__ float scaled32(float x, float2 inv) {
-    const float y = __fmul_rz(x, inv.x);
-    const float e = __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y));
-    const float cut = __fadd_rz(y, e);
-    return __uint_as_float(__float_as_uint(cut) | (e != cut - y ? 1u : 0u));
+
+// The e4m3 byte of x over a block of maximum a (448 2^-126 at least), given the
+// bytes of two values that enclose the quotient: neighbours at most, as the
+// enclosure is far narrower than their distance.
+__device__ __forceinline__ uint32_t nearer_e4m3(float x, float a, uint32_t lo, uint32_t hi) {
+    if (lo == hi) return lo;
+    const uint32_t exponent = (lo >> 3) & 15, digits = exponent ? 8 + (lo & 7) : lo & 7;
+    // t = (2 digits + 1) 2^(max(exponent, 1) - 11)
+    const float t = static_cast<float>(2 * digits + 1) * __uint_as_float((max(exponent, 1u) + 116) << 23);
+    // by a power of two, so that neither the products nor their last bits leave the range of floats
+    const float by = a >= 1.f ? 0x1p-16f : 0x1p64f;
+    const float sx = fabsf(x) * by, sa = a * by;
+    // 448 x - t a: the leading parts are near each other, and all four are multiples of 2^-5 of their last bit
+    const float px = __fmul_rn(kE4Max, sx), pa = __fmul_rn(t, sa);
+    const float diff = __fadd_rn(__fadd_rn(px, -pa), __fadd_rn(__fmaf_rn(kE4Max, sx, -px), -__fmaf_rn(t, sa, -pa)));
+    return diff > 0.f || (diff == 0.f && (lo & 1)) ? hi : lo;
 }
 
 // Two values as e4m3, to nearest, ties to even, clamped to +-448; the first in the low byte.
@@ -124,20 +134,22 @@ struct Lane {
         float f[V];
         unpack(u, f);
         if constexpr (E == Elem::kF32) {
-            // between these two products lies the exact one; a tie between them is rare
-            const float lo = inv.x * (1.0f - 0x1p-22f), hi = inv.x * (1.0f + 0x1p-22f);
+            // between these two products lies the exact one; a midpoint between them is rare
+            const float lo = inv.x * (1.0f - 0x1p-21f), hi = inv.x * (1.0f + 0x1p-21f);
             w[0] = to_e4m3x2(f[0] * lo, f[1] * lo) | to_e4m3x2(f[2] * lo, f[3] * lo) << 16;
             const uint32_t v = to_e4m3x2(f[0] * hi, f[1] * hi) | to_e4m3x2(f[2] * hi, f[3] * hi) << 16;
             if (w[0] == v) return;
+            uint32_t q = 0u;
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = scaled32(f[i], inv);
+            for (int i = 0; i < V; ++i) q |= nearer_e4m3(f[i], inv.y, (w[0] >> (8 * i)) & 255, (v >> (8 * i)) & 255) << (8 * i);
+            w[0] = q;
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) f[i] = scaled16(f[i], inv);
-        }
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i)
-            w[i] = to_e4m3x2(f[4 * i], f[4 * i + 1]) | to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16;
+            for (int i = 0; i < V / 4; ++i)
+                w[i] = to_e4m3x2(f[4 * i], f[4 * i + 1]) | to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16;
+        }
     }
     // A whole block's values as the two loads took them: from column l of it.
     static __device__ __forceinline__ void store_whole(uint8_t* block, int l, const uint4& u, float2 inv) {
@@ -157,21 +169,26 @@ struct Lane {
     }
 };
 
-// A block's scale and its reciprocal (r, d) from the bits of its maximum.
+// A block's scale from the bits of its maximum a, and what the conversion needs of
+// its reciprocal: r, and d (16 bits) or a (fp32, at least 448 2^-126).
+template <Elem E>
 __device__ __forceinline__ float block_scale(uint32_t max_bits, float2& inv) {
     const float a = __uint_as_float(max_bits);
-    constexpr float kLeast = 1.17549435e-38f;  // 2^-126
+    constexpr float kLeast = 0x1p-126f;
     if (a == 0.f) {
-        inv = make_float2(1.f, 0.f);
+        inv = make_float2(1.f, E == Elem::kF32 ? kE4Max : 0.f);
         return 1.f;
     }
     const float s = a / kE4Max;
     if (s < kLeast) {
-        inv = make_float2(8.507059e37f, 0.f);  // 2^126
+        inv = make_float2(0x1p126f, E == Elem::kF32 ? kE4Max * kLeast : 0.f);
         return kLeast;
     }
     const float r = __fdiv_rz(kE4Max, a);
-    inv = make_float2(r, isinf(a) ? 0.f : __fmaf_rn(-r, a, kE4Max) / a);  // a NaN stays
+    if constexpr (E == Elem::kF32)
+        inv = make_float2(r, a);
+    else
+        inv = make_float2(r, isinf(a) ? 0.f : __fmaf_rn(-r, a, kE4Max) / a);  // a NaN stays
     return s;
 }
 
@@ -227,7 +244,7 @@ __device__ __forceinline__ void quantize_rows_group(const QuantE4Params& p, int6
         }
     }
     float2 inv;
-    const float s = block_scale(top, inv);
+    const float s = block_scale<E>(top, inv);
     if (lane < rows) p.scale[b * p.ld_scale + first + lane] = s;
 #pragma unroll
     for (int i = 0; i < kGroup<E>; ++i) {
@@ -300,7 +317,7 @@ __device__ __forceinline__ void quantize_tile(const QuantE4Params& p, int64_t fi
     __syncthreads();
     m = __reduce_max_sync(0xffffffffu, part[lane & (kTileWarps - 1)]);
     float2 inv;
-    const float s = block_scale(m, inv);
+    const float s = block_scale<E>(m, inv);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         if constexpr (P == Part::kAligned) {

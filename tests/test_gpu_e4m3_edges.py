@@ -1,10 +1,11 @@
-"""The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes."""
+"""The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, and
+values at and beside ties."""
 
 import numpy as np
 import pytest
 
 import e4m3_reference as ref
-from test_gpu_e4m3 import DT, call, status, tdt
+from test_gpu_e4m3 import DT, call, quantize, status, tdt
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,52 @@ def test_rows_of_more_than_2_31_bytes(cuda, tiles, dtype, K, rows, pad, offset):
         s = scale[:, col // 128:-(-end // 128)] if tiles else scale[col // 128:-(-end // 128)].t()
         assert np.array_equal(s.cpu().numpy(), want_s)
         assert np.array_equal(got[:, col:end].cpu().numpy(), want_q)
+
+
+def midpoints():
+    """Every value halfway between two neighbouring e4m3 values."""
+    v = ref.decode(np.arange(0x7F))
+    return (v[1:] + v[:-1]) / 2
+
+
+def tie_rows(rng, rows, bits, exponents, share):
+    """fp32 rows of 128 values; `share` of them have one maximum a = 7 m 2^s (m of up to `bits` bits): x = t a / 448 for
+    midpoints t, which is an fp32 number where t and m have 24 bits together; every third moved to a neighbour of it."""
+    x = np.zeros((rows, 128), dtype=np.float32)
+    for r in range(rows):
+        if r % share == 0:
+            m = int(rng.integers(1, 1 << int(rng.integers(1, bits + 1)))) | 1
+            a = np.ldexp(7.0 * m, int(rng.integers(*exponents)))
+        t = rng.choice(midpoints(), 128)
+        row = (t * (a / 448)).astype(np.float32)
+        move = rng.integers(-2, 3, 128) * (rng.random(128) < 1 / 3)
+        row = np.where(move < 0, np.nextafter(row, np.float32(0)), np.where(move > 0, np.nextafter(row, np.float32(np.inf)), row))
+        row = np.minimum(row, np.float32(a)) * np.where(rng.random(128) < 0.5, -1, 1).astype(np.float32)
+        row[int(rng.integers(128))] = a
+        x[r] = row
+    return x
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("exponents", [(-15, -5), (-100, -80), (80, 104), (-3, 4)])
+def test_float32_ties(cuda, tiles, exponents):
+    """Quotients that are exact ties, and their neighbours, at ordinary, tiny and huge maxima: the bytes of the exact
+    quotient, ties to even."""
+    torch = cuda
+    x = tie_rows(np.random.default_rng(5), 2048, 20, exponents, 128 if tiles else 1)
+    q, s = quantize(torch, torch.from_numpy(x).cuda(), tiles)
+    want_q, want_s = ref.quantize(x, 128 if tiles else 1)
+    assert np.array_equal(s if tiles else s.T, want_s)
+    assert np.array_equal(q, want_q), (q != want_q).sum()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_the_same_values_give_the_same_bytes(cuda, tiles, dtype):
+    """16-bit values, ties among them, and the same values as float32."""
+    torch = cuda
+    x = tie_rows(np.random.default_rng(6), 2048, 6 if dtype == "f16" else 3, (-6, -1), 128 if tiles else 1)
+    x = torch.from_numpy(x).cuda().to(tdt(torch, dtype))
+    q, s = quantize(torch, x, tiles)
+    q32, s32 = quantize(torch, x.float(), tiles)
+    assert np.array_equal(s, s32) and np.array_equal(q, q32), (q != q32).sum()
