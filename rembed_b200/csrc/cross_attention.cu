@@ -87,11 +87,6 @@ struct Const {
 // registers of the two-tile kernel: 128 * 72 + 256 * 216 = 384 * 168
 constexpr int kControlRegs = 72, kSoftmaxRegs = 216;
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Pairs of floats in one 64-bit register: half the instructions.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     uint64_t r;
@@ -506,7 +501,8 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         // rows of out on 32-byte boundaries: a thread stores whole sectors
         const bool sectors = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % 16 == 0;
         uint32_t cn = 0, on = 0;        // blocks and outputs of this tile so far
-        float m = -INFINITY, l = 0.f;   // this row's maximum (exp2 domain) and sum
+        // this row's maximum (a score, and times scale) and sum
+        float m = -INFINITY, ms = -INFINITY, l = 0.f;
         Work w = {};  // split: still there for the join
         bool done = true;
         for (uint32_t k = 0; done; ++k) {
@@ -514,7 +510,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             if (next.h < 0) break;
             w = next;
             if (t >= w.nt) continue;
-            m = -INFINITY;
+            m = ms = -INFINITY;
             l = 0.f;
             if (w.nb > 0) {
                 const uint32_t zero[16] = {};
@@ -546,30 +542,47 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
 #pragma unroll
                 for (int j = 8; j < BKV; j += 2)
                     pm[(j >> 1) & 7] = max3(pm[(j >> 1) & 7], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
-                const float mx =
-                    max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], pm[7])) * scale;
-                // The maximum in use stays until a block's is more than 8 above it:
-                // P is at most 2^8, O is rescaled rarely, and the division by the sum
-                // cancels it.  A NaN or +infinity among the scores makes the row NaN.
-                const float now = mx > m + 8.0f ? mx : m;
-                const float off = mx < INFINITY ? (now == -INFINITY ? 0.f : -now) : mx - mx;
-                const float alpha = exp2_approx(m + off);
-                m = now;
-                if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                    if (NS == 2) {
-                        done = mbar_wait_warp(&ofull[t * NS + (cn - 1) % NS], ((cn - 1) / NS) & 1, p.status, abort_flag);
-                        if (!done) break;
-                        tc_fence_after();
-                    }
+                const float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], pm[7]));
+                // The maximum in use stays until a block's is more than 8 above it in
+                // the exponent: P is at most 2^8, O is rescaled rarely, and the division
+                // by the sum cancels it.  A NaN or +infinity among the scores makes the
+                // row NaN.
+                const float mxs = __fmul_rn(mx, scale);
+                const bool up = mxs > ms + 8.0f;
+                const float now = up ? mxs : ms;
+                float off = mx < INFINITY ? -now : mx - mx;
+                float alpha = ex2(ms + off);
+                const bool far = fabsf(now) > kFar;
+                if (__any_sync(0xffffffffu, alpha != 1.0f || far)) {
+                    if (far) {  // hardly ever
+                        far_maximum(mx, scale, m, ms, alpha);
+                        if (mx < INFINITY) off = 0.f;
+                        if (m > -INFINITY) {
 #pragma unroll
-                    for (int j = 0; j < D; j += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(tO + j, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st16(tO + j, o);
+                            for (int j = 0; j < BKV; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) - m);
+                        }
                     }
+                    __syncwarp();
+                    if (i > 0) {
+                        if (NS == 2) {
+                            done = mbar_wait_warp(&ofull[t * NS + (cn - 1) % NS], ((cn - 1) / NS) & 1, p.status, abort_flag);
+                            if (!done) break;
+                            tc_fence_after();
+                        }
+#pragma unroll
+                        for (int j = 0; j < D; j += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + j, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st16(tO + j, o);
+                        }
+                    }
+                }
+                if (!far) {
+                    m = up ? mx : m;
+                    ms = now;
                 }
                 const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
                 uint64_t sum2[2] = {0, 0};
@@ -584,8 +597,8 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                         if (e % S::FMA_EVERY == S::FMA_EVERY - 1) {
                             exp2_fma(a, b);
                         } else {
-                            a = exp2_approx(a);
-                            b = exp2_approx(b);
+                            a = ex2(a);
+                            b = ex2(b);
                         }
                         sum2[e & 1] = add_pair(sum2[e & 1], pair_of(a, b));
                         // rounded to the 16 bits of V for the product, by at most half a step
@@ -670,7 +683,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    f[k] = f[k] == -INFINITY ? 0.f : exp2_approx(f[k] - top);
+                    f[k] = f[k] == -INFINITY ? 0.f : ex2(reference_step(f[k], top, scale));
                     if (k < split) sum += f[k] * ld_shared_cluster(mapa_shared(smem_u32(sL + t * 128 + r), k));
                 }
                 const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);

@@ -46,6 +46,37 @@ __device__ __forceinline__ bool cross_seq(const CrossParams& p, int s, CrossSeq&
     if (!ok && raise) atomicOr(p.status, raise);
     return ok;
 }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A key's exponent is its score x times scale less its row's reference, which is the
+// same for all of the row's keys and cancels.  While the score m in use for the
+// maximum has |m scale| up to 2^10, the reference is that product, rounded.
+// Beyond, the rounding would come to reach the size of the exponents, or the
+// product is not finite: there it is the exact product, and the exponent (x - m)
+// scale.  A row that goes from one to the other mixes exponents 2^-14 apart.
+constexpr float kFar = 0x1p10f;
+// The maximum of a row's next keys, mx, into m and mscaled = m scale (rounded), where
+// the larger of the two is far; weights so far count alpha times from here on.
+__device__ __forceinline__ void far_maximum(float mx, float scale, float& m, float& mscaled, float& alpha) {
+    const bool near = fabsf(mscaled) <= kFar;
+    const float up = (mx - m) * scale;
+    alpha = 1.0f;
+    if (near || up > 8.0f) {
+        alpha = ex2(near ? mscaled - mx * scale : -up);
+        m = mx;
+        mscaled = mx * scale;
+    }
+}
+// By how much the exponents over m = a are above those over m = b.
+__device__ __forceinline__ float reference_step(float a, float b, float scale) {
+    const float sa = __fmul_rn(a, scale), sb = __fmul_rn(b, scale);
+    return fabsf(sa) > kFar && fabsf(sb) > kFar ? (a - b) * scale : sa - sb;
+}
 #endif
 
 // What a kernel would do with a call: CTAs before the keys are split, and over

@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "act16.cuh"
 #include "clusters.cuh"
 #include "cross_attention.cuh"
@@ -74,11 +76,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, int split) {
@@ -122,8 +119,11 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto begin = [&]() {
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(first + i * step, i);
+        for (int i = 0; i < STAGES - 1; ++i) load(first + i * step, i);
+    };
+    begin();
 
     // Q as A fragments: rows lane / 4 and lane / 4 + 8 of the tile
     uint32_t qa[D / 16][4];
@@ -143,90 +143,123 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int stage = 0;
-    for (int chunk = first; chunk < chunks; chunk += step) {
-        load(chunk + (STAGES - 1) * step, (stage + STAGES - 1) % STAGES);
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // a row's maximum (a score) and sum
+    // All chunks, with references that are rounded products or exact ones (see kFar).
+    // A row of the former whose farthest maximum was too far has to be gone
+    // through again: a test in the loop, in front of the exponentials, cost 4 to 15%.
+    float farthest = 0.f;
+    auto walk = [&](auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
+        float ms[2] = {-INFINITY, -INFINITY};  // m times scale
+        int stage = 0;
+        for (int chunk = first; chunk < chunks; chunk += step) {
+            load(chunk + (STAGES - 1) * step, (stage + STAGES - 1) % STAGES);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            __syncwarp();
+            const uint32_t kb = ring + stage * 2 * CHUNK, vb = kb + CHUNK;
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) {  // 32 of D: four 8 x 8 pieces of eight keys
+                    uint32_t b[4];
+                    ldsm4(b, kb + piece<D>(n * 8 + (lane & 7), k * 4 + (lane >> 3)));
+                    mma16816<F16>(sc[n], qa[2 * k], b[0], b[1]);
+                    mma16816<F16>(sc[n], qa[2 * k + 1], b[2], b[3]);
+                }
+            }
+            if ((chunk + 1) * KEYS > c.nk) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (chunk * KEYS + n * 8 + (lane & 3) * 2 + (e & 1) >= c.nk) sc[n][e] = -INFINITY;
+            }
+            // The maximum in use stays until a chunk's is more than 8 above it in the
+            // exponent (P is then at most 2^8; the final division cancels it).
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1]));
+                mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
+            }
+            float alpha[2], off[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                if constexpr (EXACT) {
+                    const float up = (mx[h] - m[h]) * p.scale_log2;
+                    alpha[h] = up > 8.0f ? ex2(-up) : 1.0f;
+                    m[h] = up > 8.0f ? mx[h] : m[h];
+                    off[h] = 0.f;
+                    if (m[h] > -INFINITY) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            sc[n][2 * h] -= m[h];
+                            sc[n][2 * h + 1] -= m[h];
+                        }
+                    }
+                } else {
+                    const float mxs = __fmul_rn(mx[h], p.scale_log2);
+                    const bool up = mxs > ms[h] + 8.0f;
+                    off[h] = up ? -mxs : -ms[h];
+                    alpha[h] = ex2(ms[h] + off[h]);
+                    m[h] = up ? mx[h] : m[h];
+                    ms[h] = -off[h];
+                    farthest = fmaxf(farthest, fabsf(mxs));
+                }
+            }
+            float add[2] = {0.f, 0.f};
+            uint32_t pa[NT / 2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] = ex2(fmaf(sc[n][e], p.scale_log2, off[e >> 1]));
+                add[0] += sc[n][0] + sc[n][1];
+                add[1] += sc[n][2] + sc[n][3];
+                // P is rounded to the 16 bits of V for the product: an element by at
+                // most half a step, as V's own values were
+                pa[n / 2][(n & 1) * 2] = pack2<F16>(sc[n][0], sc[n][1]);
+                pa[n / 2][(n & 1) * 2 + 1] = pack2<F16>(sc[n][2], sc[n][3]);
+            }
+            l[0] = l[0] * alpha[0] + add[0];
+            l[1] = l[1] * alpha[1] + add[1];
+            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    o[i][0] *= alpha[0];
+                    o[i][1] *= alpha[0];
+                    o[i][2] *= alpha[1];
+                    o[i][3] *= alpha[1];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NT / 2; ++k) {  // 16 keys
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {  // 16 of D: keys 0-7 and 8-15 of two eights
+                    uint32_t b[4];
+                    ldsm4_t(b, vb + piece<D>(k * 16 + (lane & 15), i * 2 + (lane >> 4)));
+                    mma16816<F16>(o[2 * i], pa[k], b[0], b[1]);
+                    mma16816<F16>(o[2 * i + 1], pa[k], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
-        const uint32_t kb = ring + stage * 2 * CHUNK, vb = kb + CHUNK;
-        float sc[NT][4];
+    };
+    walk(std::false_type{});
+    if (__any_sync(0xffffffffu, farthest > kFar)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {  // 32 of D: four 8 x 8 pieces of eight keys
-                uint32_t b[4];
-                ldsm4(b, kb + piece<D>(n * 8 + (lane & 7), k * 4 + (lane >> 3)));
-                mma16816<F16>(sc[n], qa[2 * k], b[0], b[1]);
-                mma16816<F16>(sc[n], qa[2 * k + 1], b[2], b[3]);
-            }
-        }
-        if ((chunk + 1) * KEYS > c.nk) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (chunk * KEYS + n * 8 + (lane & 3) * 2 + (e & 1) >= c.nk) sc[n][e] = -INFINITY;
-        }
-        // Scores in the exp2 domain; the maximum in use stays until a chunk's is
-        // more than 8 above it (P is then at most 2^8; the final division cancels it).
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1]));
-            mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
-        }
-        float alpha[2], off[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            mx[h] *= p.scale_log2;
-            const float now = mx[h] > m[h] + 8.0f ? mx[h] : m[h];
-            off[h] = now == -INFINITY ? 0.f : -now;
-            alpha[h] = ex2(m[h] + off[h]);
-            m[h] = now;
-        }
-        float add[2] = {0.f, 0.f};
-        uint32_t pa[NT / 2][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[n][e] = ex2(fmaf(sc[n][e], p.scale_log2, off[e >> 1]));
-            add[0] += sc[n][0] + sc[n][1];
-            add[1] += sc[n][2] + sc[n][3];
-            // P is rounded to the 16 bits of V for the product: an element by at
-            // most half a step, as V's own values were
-            pa[n / 2][(n & 1) * 2] = pack2<F16>(sc[n][0], sc[n][1]);
-            pa[n / 2][(n & 1) * 2 + 1] = pack2<F16>(sc[n][2], sc[n][3]);
-        }
-        l[0] = l[0] * alpha[0] + add[0];
-        l[1] = l[1] * alpha[1] + add[1];
-        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= alpha[0];
-                o[i][1] *= alpha[0];
-                o[i][2] *= alpha[1];
-                o[i][3] *= alpha[1];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NT / 2; ++k) {  // 16 keys
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {  // 16 of D: keys 0-7 and 8-15 of two eights
-                uint32_t b[4];
-                ldsm4_t(b, vb + piece<D>(k * 16 + (lane & 15), i * 2 + (lane >> 4)));
-                mma16816<F16>(o[2 * i], pa[k], b[0], b[1]);
-                mma16816<F16>(o[2 * i + 1], pa[k], b[2], b[3]);
-            }
-        }
-        __syncwarp();
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+        begin();
+        walk(std::true_type{});
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncwarp();
 
     // this warp's part: outputs [kRows][D] in its ring, maximum and sum beside them
     float* mine = reinterpret_cast<float*>(smem + warp * S::RING);
@@ -246,7 +279,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
         }
     }
     __syncthreads();
-    // The warps' parts joined: each row's weights 2^(m - the largest m), its sum
+    // The warps' parts joined: each row's weights by its maxima, its sum
     // and maximum, then its outputs in the first warp's place.
     if (threadIdx.x < rows) {
         const int r = threadIdx.x;
@@ -255,7 +288,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
         for (int i = 1; i < kWarps; ++i) top = fmaxf(top, sM[i * kRows + r]);
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
-            const float w = sM[i * kRows + r] == -INFINITY ? 0.f : ex2(sM[i * kRows + r] - top);
+            const float w = sM[i * kRows + r] == -INFINITY ? 0.f : ex2(reference_step(sM[i * kRows + r], top, p.scale_log2));
             sW[i * kRows + r] = w;
             sum += w * sL[i * kRows + r];
         }
@@ -314,7 +347,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                     if (k < split) sum += 0.f * s[k];  // NaN stays
                     continue;
                 }
-                const float f = ex2(w[k] - top);
+                const float f = ex2(reference_step(w[k], top, p.scale_log2));
                 sum = fmaf(f, s[k], sum);
                 a = fmaf(f, x[k], a);
                 b = fmaf(f, y[k], b);

@@ -1,0 +1,127 @@
+"""rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds."""
+
+import pytest
+
+from test_gpu_cross_attention import HEADS, Batch, status
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def exact_rows(torch, b, scale):
+    """The float64 result of every row of b's first sequence, and the bound on what the kernels may be off it, for
+    scores that are exact in fp32.  With u half a step of the type and A = sum_j p_j |v_j|: probabilities and result
+    are rounded (u A and u |o|, and their product); weights above 2^-30 have exponents of at most 30, so that scale's
+    and the product's roundings (2^-24 of them each), the hardware exponential (2^-22) and the polynomial (2^-18)
+    move them by at most 2^-16 in all, and where scores pass 2^10 in the exponent its rounding there by 2^-14; the
+    sums' additions add (keys + 16) 2^-23 A, and in fp16 small probabilities keep 2^-25 absolute."""
+    D, group, n, k = b.dim, b.heads // b.kv_heads, b.ql[0], b.kl[0]
+    u = torch.finfo(b.out.dtype).eps / 2
+    want, tol = [], []
+    for h in range(b.heads):
+        j = h // group * D
+        K, V = b.kv[:k, j:j + D].double(), b.kv[:k, b.kv_heads * D + j:b.kv_heads * D + j + D].double()
+        S = b.q[:n, h * D:(h + 1) * D].double() @ K.t() * scale
+        P = torch.softmax(S, 1)
+        o, A = P @ V, P @ V.abs()
+        want.append(o)
+        tol.append(u * (A + o.abs()) + u * u * A + (2.0**-16 + 2.0**-14) * A + (k + 16) * 2.0**-23 * A + 2.0**-25 * V.abs().sum(0))
+    return torch.cat(want, 1), torch.cat(tol, 1)
+
+
+def check_exact(torch, b):
+    b.run()
+    status(torch)
+    want, tol = exact_rows(torch, b, b.scale)
+    got = b.out[:b.ql[0], :b.heads * b.dim].double()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).nan_to_num(INF).max())
+
+
+def signs(torch, n):
+    return torch.where(torch.arange(n, device="cuda") % 3 == 1, -1.0, 1.0)[:, None]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("q", [1, 5, 150])
+def test_scores_of_hundreds_of_millions(cuda, heads, kv_heads, dim, dtype, q):
+    """Finite queries and keys of several thousand: scores up to 10^9, whose products with the scale are rounded to
+    steps of 64 and more.  All the weight lies on the largest score, shared by equal ones.  Every score is exact in
+    fp32: 32 equal products of an 8- or 10-bit and a 7-bit number."""
+    torch = cuda
+    b = Batch(torch, [q], [700], heads, kv_heads, dim, dtype, 70 + dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    r = torch.randint(1, 128, (700, kv_heads), device="cuda", generator=g).float()
+    b.q.zero_()
+    b.kv[:, :kv_heads * dim] = 0
+    for h in range(heads):
+        b.q[:q, h * dim:h * dim + 32] = (signs(torch, q) * (6976.0 if dtype == "bf16" else 7000.0)).to(b.q.dtype)
+    for h in range(kv_heads):
+        b.kv[:, h * dim:h * dim + 32] = (64 * r[:, h:h + 1]).to(b.kv.dtype)
+    b.scale = 0.37
+    check_exact(torch, b)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("q", [1, 5, 150])
+@pytest.mark.parametrize("base", [2.0**11, -2.0**11, 2.0**8])
+def test_small_differences_of_large_scores(cuda, heads, kv_heads, dim, dtype, q, base):
+    """Scores of several millions (of a million: base 2^8) that differ by small whole numbers, exact in fp32, and a
+    text that begins with keys of small scores: those of larger ones take all the weight, by their differences."""
+    torch = cuda
+    b = Batch(torch, [q], [700], heads, kv_heads, dim, dtype, 80 + dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    b.q.zero_()
+    b.kv[:, :kv_heads * dim] = 0
+    for h in range(heads):
+        b.q[:q, h * dim] = 4096.0
+        b.q[:q, h * dim + 1] = 1.0
+    for h in range(kv_heads):
+        b.kv[130:, h * dim] = base
+        b.kv[:, h * dim + 1] = torch.randint(0, 16, (700,), device="cuda", generator=g).to(b.kv.dtype)
+    b.scale = 0.37
+    check_exact(torch, b)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("q", [2, 5, 150])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_pass_a_thousand(cuda, heads, kv_heads, dim, dtype, q, falling):
+    """Maxima that rise or fall through 2^10 and -2^10 in the exponent, by steps of 8.5 with differences within them."""
+    torch = cuda
+    b = Batch(torch, [q], [700], heads, kv_heads, dim, dtype, 85 + dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    b.q.zero_()
+    b.kv[:, :kv_heads * dim] = 0
+    ramp = torch.div(torch.arange(700, device="cuda") * 16, 700, rounding_mode="floor") + 112
+    for h in range(heads):
+        b.q[:q, h * dim] = 16 * signs(torch, q)[:, 0].to(b.q.dtype)
+        b.q[:q, h * dim + 1] = 1.0
+    for h in range(kv_heads):
+        b.kv[:, h * dim] = (ramp.flip(0) if falling else ramp).to(b.kv.dtype)
+        b.kv[:, h * dim + 1] = torch.randint(0, 16, (700,), device="cuda", generator=g).to(b.kv.dtype)
+    b.scale = 0.37
+    check_exact(torch, b)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("q", [1, 5, 150])
+@pytest.mark.parametrize("dtype,query,step,scale", [
+    ("bf16", 1.5 * 2.0**60, 2.0**53, 1000.0), ("bf16", 1.0, 1.0, 2.0e38), ("f16", 1.0, 1.0, 2.0e38),
+])
+def test_scores_that_overflow_with_the_scale(cuda, heads, kv_heads, dim, q, dtype, query, step, scale):
+    """Finite scores whose product with an allowed scale is none in fp32: the largest takes all the weight."""
+    torch = cuda
+    b = Batch(torch, [q], [300], heads, kv_heads, dim, dtype, 90 + dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    b.q.zero_()
+    b.kv[:, :kv_heads * dim] = 0
+    for h in range(heads):
+        b.q[:q, h * dim] = (signs(torch, q)[:, 0] * query).to(b.q.dtype)
+    for h in range(kv_heads):
+        b.kv[:, h * dim] = (step * torch.randint(2, 128, (300,), device="cuda", generator=g).float()).to(b.kv.dtype)
+    b.scale = scale
+    check_exact(torch, b)
