@@ -311,7 +311,7 @@ int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, c
  * output is zeros.  Rows of out outside every sequence are left alone.  Scores
  * are fp32 sums of products; finite ones may be of any size, their product with
  * scale too (the largest then takes all the weight).  A row with a NaN or
- * +infinity among its scores is NaN.
+ * +infinity among its scores, or with nothing but -infinities, is NaN.
  *
  * Heads as in rg_attention: query head h at columns h * head_dim, key/value
  * head h / (heads / kv_heads); head dims 32, 64, 128, 256; dtype

@@ -109,7 +109,9 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 // 2^x of a pair on the FMA pipe: n = round(x) by the magic constant 1.5 * 2^23,
 // 2^f on [-1/2, 1/2] by a quartic fitted here for least relative error (2.7e-6
 // in fp32), n added to the exponent.  Clamped at 2^-125, which is nothing beside
-// a sum of at least one; a row with a NaN or +infinity is NaN already (below).
+// a sum of at least one: a row's maximum is its reference or up to 2^8 above.  A
+// row without such a maximum comes out by row_weight, and what it has gathered
+// counts 0 times once it finds one; a row with a NaN or +infinity is NaN already.
 __device__ __forceinline__ void exp2_fma(float& a, float& b) {
     const uint64_t x = pair_of(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
     const uint64_t magic = pair_of(12582912.0f, 12582912.0f);
@@ -141,6 +143,7 @@ struct Work {
     int k0, nb;        // first row of k and v, blocks of keys
     int tail;          // keys of the last of the nb blocks
     int clear;         // it ends within a 16-key step
+    int keys;          // the sequence has keys
 };
 
 template <int D>
@@ -163,6 +166,7 @@ __device__ __forceinline__ Work work_of(const CrossParams& p, int item, int qtil
     w.nb = b1 - b0;
     w.tail = b1 == blocks ? c.nk - (blocks - 1) * S::BKV : S::BKV;
     w.clear = w.nb > 0 && (w.tail & 15) != 0;
+    w.keys = c.nk > 0;
     return w;
 }
 
@@ -625,7 +629,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             if (!done) break;
             tc_fence_after();
             if (split == 1) {
-                const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+                const float inv = row_weight(m, l, w.keys);
                 uint16_t* out = p.out + static_cast<int64_t>(w.row + t * 128 + r) * p.ldo + w.h * D;
 #pragma unroll
                 for (int j = 0; j < D; j += 16) {
@@ -686,7 +690,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     f[k] = f[k] == -INFINITY ? 0.f : ex2(reference_step(f[k], top, scale));
                     if (k < split) sum += f[k] * ld_shared_cluster(mapa_shared(smem_u32(sL + t * 128 + r), k));
                 }
-                const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+                const float inv = row_weight(top, sum, w.keys);
                 uint16_t* out = p.out + static_cast<int64_t>(w.row + t * 128 + r) * p.ldo + w.h * D;
                 for (int j = rank * (D / split); j < (rank + 1) * (D / split); j += 8) {
                     float v[8];

@@ -77,6 +77,11 @@ __device__ __forceinline__ float reference_step(float a, float b, float scale) {
     const float sa = __fmul_rn(a, scale), sb = __fmul_rn(b, scale);
     return fabsf(sa) > kFar && fabsf(sb) > kFar ? (a - b) * scale : sa - sb;
 }
+// What a row's products are multiplied by at the end, from its maximum and sum: no
+// key gives zeros, keys with scores of -infinity alone 0 / 0; a NaN stays.
+__device__ __forceinline__ float row_weight(float m, float sum, bool keys) {
+    return m > -INFINITY ? 1.0f / sum : __int_as_float(keys ? 0x7fffffff : 0);
+}
 #endif
 
 // What a kernel would do with a call: CTAs before the keys are split, and over

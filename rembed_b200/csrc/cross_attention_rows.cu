@@ -322,13 +322,15 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
     else __syncthreads();
     for (int e = rank * 32 * kWarps + threadIdx.x; e < rows * (D / 2); e += split * 32 * kWarps) {
         const int r = e / (D / 2), d = (e % (D / 2)) * 2;
-        float a, b, sum;
+        float a, b, sum, top;
         if (split == 1) {
             a = joined[2 * e];
             b = joined[2 * e + 1];
             sum = sSum[r];
+            top = sTop[r];
         } else {
-            float w[8], s[8], x[8], y[8], top = -INFINITY;
+            float w[8], s[8], x[8], y[8];
+            top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t to = k < split ? k : 0;
@@ -353,7 +355,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                 b = fmaf(f, y[k], b);
             }
         }
-        const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // no key: zeros; NaN stays
+        const float inv = row_weight(top, sum, c.nk > 0);
         const int row = tile * kRows + r;
         uint16_t* out = p.out + static_cast<int64_t>(c.q0 + row / p.group) * p.ldo + (hk * p.group + row % p.group) * D + d;
         *reinterpret_cast<uint32_t*>(out) = pack2<F16>(a * inv, b * inv);

@@ -1,4 +1,5 @@
-"""rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds."""
+"""rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds, and rows
+whose every score is -infinity."""
 
 import pytest
 
@@ -125,3 +126,57 @@ def test_scores_that_overflow_with_the_scale(cuda, heads, kv_heads, dim, q, dtyp
         b.kv[:, h * dim] = (step * torch.randint(2, 128, (300,), device="cuda", generator=g).float()).to(b.kv.dtype)
     b.scale = scale
     check_exact(torch, b)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("q", [3, 150])
+def test_rows_of_minus_infinities(cuda, heads, kv_heads, dim, dtype, q):
+    """Keys that hold an infinity, met by negative queries.  Where a text has no other key the softmax is 0 / 0: NaN, of
+    one key as of many, and for every place in a block.  Where it has others, the result is theirs."""
+    torch = cuda
+    kl = [1, 3, 140, 300, 50]
+    hidden = [range(1), range(3), range(140), range(260), range(0)]  # the keys with an infinity
+    b = Batch(torch, [q] * len(kl), kl, heads, kv_heads, dim, dtype, 50 + dim)
+    b.q[:, :heads * dim:dim] = -b.q[:, :heads * dim:dim].abs() - 0.5
+    clean = b.run().clone()
+    for at, keys in zip(b.begin, hidden):
+        if len(keys):
+            b.kv[at + keys[0]:at + keys[-1] + 1, :kv_heads * dim:dim] = INF
+    b.out.fill_(-7.0)
+    got = b.run()[:, :heads * dim]
+    status(torch)
+    assert bool(torch.isnan(got[:3 * q]).all())
+    assert torch.equal(got[4 * q:5 * q], clean[4 * q:5 * q, :heads * dim])
+    rest = Batch(torch, [0, 0, 0, q, 0], kl, heads, kv_heads, dim, dtype, 1)
+    rest.q, rest.kv, rest.Tq = b.q[3 * q:].contiguous(), b.kv, q + 3
+    rest.begin[3] += 260
+    rest.kl[3] -= 260
+    rest.tables[1][3] += 260
+    rest.tables[2][3] -= 260
+    rest.out = torch.full((q + 3, heads * dim + 16), -7.0, device="cuda", dtype=b.out.dtype)
+    rest.run()
+    status(torch)
+    rest.check()
+    # the same weights from sums in another order: within what both may be off the exact result
+    v = b.kv[b.begin[3]:b.begin[3] + 300, kv_heads * dim:].float().abs().max()
+    u = torch.finfo(b.out.dtype).eps / 2
+    assert float((got[3 * q:4 * q].float() - rest.out[:q, :heads * dim].float()).abs().max()) <= 4 * u * float(v)
+
+
+@pytest.mark.parametrize("q,keys,heads,kv_heads,dim", [
+    (1, 9000, 1, 1, 128), (1, 5000, 2, 1, 256), (3, 20000, 4, 1, 64), (130, 6000, 1, 1, 128), (300, 5000, 2, 1, 256),
+    (200, 4100, 2, 2, 64), (500, 8000, 1, 1, 32),
+])
+def test_minus_infinities_in_split_keys(cuda, q, keys, heads, kv_heads, dim):
+    """The same where the keys are split over a cluster: all parts without weight (NaN), then all but the last key's."""
+    torch = cuda
+    b = Batch(torch, [q], [keys], heads, kv_heads, dim, "bf16", 60 + dim)
+    b.q[:, :heads * dim:dim] = -b.q[:, :heads * dim:dim].abs() - 0.5
+    b.kv[:, :kv_heads * dim:dim] = INF
+    assert bool(torch.isnan(b.run()[:q, :heads * dim]).all())
+    b.kv[keys - 1, :kv_heads * dim:dim] = 1.0
+    got = b.run()[:q, :heads * dim]
+    status(torch)
+    v = b.kv[keys - 1, kv_heads * dim:].view(kv_heads, 1, dim).expand(kv_heads, heads // kv_heads, dim).reshape(1, -1)
+    assert torch.equal(got, v.expand(q, -1))
