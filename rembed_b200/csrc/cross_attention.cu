@@ -505,8 +505,8 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
         // rows of out on 32-byte boundaries: a thread stores whole sectors
         const bool sectors = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.ldo % 16 == 0;
         uint32_t cn = 0, on = 0;        // blocks and outputs of this tile so far
-        // this row's maximum (a score, and times scale) and sum
-        float m = -INFINITY, ms = -INFINITY, l = 0.f;
+        // this row's maximum (a score), its reference, and sum
+        float m = -INFINITY, ref = -INFINITY, l = 0.f;
         Work w = {};  // split: still there for the join
         bool done = true;
         for (uint32_t k = 0; done; ++k) {
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
             if (next.h < 0) break;
             w = next;
             if (t >= w.nt) continue;
-            m = ms = -INFINITY;
+            m = ref = -INFINITY;
             l = 0.f;
             if (w.nb > 0) {
                 const uint32_t zero[16] = {};
@@ -548,19 +548,19 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                     pm[(j >> 1) & 7] = max3(pm[(j >> 1) & 7], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
                 const float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], pm[7]));
                 // The maximum in use stays until a block's is more than 8 above it in
-                // the exponent: P is at most 2^8, O is rescaled rarely, and the division
-                // by the sum cancels it.  A NaN or +infinity among the scores makes the
+                // the exponent: P is at most 2^8 (fp16 2^15), O is rescaled rarely, and the
+                // division by the sum cancels it.  A NaN or +infinity among the scores makes the
                 // row NaN.
-                const float mxs = __fmul_rn(mx, scale);
-                const bool up = mxs > ms + 8.0f;
-                const float now = up ? mxs : ms;
+                const float mxr = reference<F16>(mx, scale);
+                const bool up = mxr > ref + 8.0f;
+                const float now = up ? mxr : ref;
                 float off = mx < INFINITY ? -now : mx - mx;
-                float alpha = ex2(ms + off);
+                float alpha = ex2(ref + off);
                 const bool far = fabsf(now) > kFar;
                 if (__any_sync(0xffffffffu, alpha != 1.0f || far)) {
                     if (far) {  // hardly ever
-                        far_maximum(mx, scale, m, ms, alpha);
-                        if (mx < INFINITY) off = 0.f;
+                        far_maximum<F16>(mx, scale, m, ref, alpha);
+                        if (mx < INFINITY) off = kLift<F16>;
                         if (m > -INFINITY) {
 #pragma unroll
                             for (int j = 0; j < BKV; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) - m);
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
                 if (!far) {
                     m = up ? mx : m;
-                    ms = now;
+                    ref = now;
                 }
                 const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
                 uint64_t sum2[2] = {0, 0};
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(TileShape<D>::THREADS, 1)
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    f[k] = f[k] == -INFINITY ? 0.f : ex2(reference_step(f[k], top, scale));
+                    f[k] = f[k] == -INFINITY ? 0.f : ex2(reference_step<F16>(f[k], top, scale));
                     if (k < split) sum += f[k] * ld_shared_cluster(mapa_shared(smem_u32(sL + t * 128 + r), k));
                 }
                 const float inv = row_weight(top, sum, w.keys);

@@ -59,23 +59,34 @@ __device__ __forceinline__ float ex2(float x) {
 // Beyond, the rounding would come to reach the size of the exponents, or the
 // product is not finite: there it is the exact product, and the exponent (x - m)
 // scale.  A row that goes from one to the other mixes exponents 2^-14 apart.
+// fp16 has no steps below 2^-24, and a long text many probabilities down there:
+// its exponents are 7 higher (probabilities up to 2^15; 8 of that is how far a
+// maximum may be above the one in use).
 constexpr float kFar = 0x1p10f;
-// The maximum of a row's next keys, mx, into m and mscaled = m scale (rounded), where
-// the larger of the two is far; weights so far count alpha times from here on.
-__device__ __forceinline__ void far_maximum(float mx, float scale, float& m, float& mscaled, float& alpha) {
-    const bool near = fabsf(mscaled) <= kFar;
+template <bool F16>
+constexpr float kLift = F16 ? 7.0f : 0.0f;
+template <bool F16>
+__device__ __forceinline__ float reference(float m, float scale) {
+    return F16 ? __fmaf_rn(m, scale, -kLift<F16>) : __fmul_rn(m, scale);
+}
+// The maximum of a row's next keys, mx, into m and its reference ref, where the
+// larger one's reference is far; weights so far count alpha times from here on.
+template <bool F16>
+__device__ __forceinline__ void far_maximum(float mx, float scale, float& m, float& ref, float& alpha) {
+    const bool near = fabsf(ref) <= kFar;
     const float up = (mx - m) * scale;
     alpha = 1.0f;
     if (near || up > 8.0f) {
-        alpha = ex2(near ? mscaled - mx * scale : -up);
+        alpha = ex2(near ? ref - reference<F16>(mx, scale) : -up);
         m = mx;
-        mscaled = mx * scale;
+        ref = reference<F16>(mx, scale);
     }
 }
-// By how much the exponents over m = a are above those over m = b.
+// By how much the reference of m = a is above that of m = b.
+template <bool F16>
 __device__ __forceinline__ float reference_step(float a, float b, float scale) {
-    const float sa = __fmul_rn(a, scale), sb = __fmul_rn(b, scale);
-    return fabsf(sa) > kFar && fabsf(sb) > kFar ? (a - b) * scale : sa - sb;
+    const float ra = reference<F16>(a, scale), rb = reference<F16>(b, scale);
+    return fabsf(ra) > kFar && fabsf(rb) > kFar ? (a - b) * scale : ra - rb;
 }
 // What a row's products are multiplied by at the end, from its maximum and sum: no
 // key gives zeros, keys with scores of -infinity alone 0 / 0; a NaN stays.

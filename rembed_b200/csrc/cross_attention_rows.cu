@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
     float farthest = 0.f;
     auto walk = [&](auto exact) {
         constexpr bool EXACT = decltype(exact)::value;
-        float ms[2] = {-INFINITY, -INFINITY};  // m times scale
+        float ref[2] = {-INFINITY, -INFINITY};  // of m
         int stage = 0;
         for (int chunk = first; chunk < chunks; chunk += step) {
             load(chunk + (STAGES - 1) * step, (stage + STAGES - 1) % STAGES);
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                         if (chunk * KEYS + n * 8 + (lane & 3) * 2 + (e & 1) >= c.nk) sc[n][e] = -INFINITY;
             }
             // The maximum in use stays until a chunk's is more than 8 above it in the
-            // exponent (P is then at most 2^8; the final division cancels it).
+            // exponent (P is then at most 2^8, fp16 2^15; the final division cancels it).
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                     const float up = (mx[h] - m[h]) * p.scale_log2;
                     alpha[h] = up > 8.0f ? ex2(-up) : 1.0f;
                     m[h] = up > 8.0f ? mx[h] : m[h];
-                    off[h] = 0.f;
+                    off[h] = kLift<F16>;
                     if (m[h] > -INFINITY) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
@@ -202,13 +202,13 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                         }
                     }
                 } else {
-                    const float mxs = __fmul_rn(mx[h], p.scale_log2);
-                    const bool up = mxs > ms[h] + 8.0f;
-                    off[h] = up ? -mxs : -ms[h];
-                    alpha[h] = ex2(ms[h] + off[h]);
+                    const float mxr = reference<F16>(mx[h], p.scale_log2);
+                    const bool up = mxr > ref[h] + 8.0f;
+                    off[h] = up ? -mxr : -ref[h];
+                    alpha[h] = ex2(ref[h] + off[h]);
                     m[h] = up ? mx[h] : m[h];
-                    ms[h] = -off[h];
-                    farthest = fmaxf(farthest, fabsf(mxs));
+                    ref[h] = -off[h];
+                    farthest = fmaxf(farthest, fabsf(mxr));
                 }
             }
             float add[2] = {0.f, 0.f};
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
         for (int i = 1; i < kWarps; ++i) top = fmaxf(top, sM[i * kRows + r]);
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
-            const float w = sM[i * kRows + r] == -INFINITY ? 0.f : ex2(reference_step(sM[i * kRows + r], top, p.scale_log2));
+            const float w = sM[i * kRows + r] == -INFINITY ? 0.f : ex2(reference_step<F16>(sM[i * kRows + r], top, p.scale_log2));
             sW[i * kRows + r] = w;
             sum += w * sL[i * kRows + r];
         }
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_rows_kernel(CrossParams p, 
                     if (k < split) sum += 0.f * s[k];  // NaN stays
                     continue;
                 }
-                const float f = ex2(reference_step(w[k], top, p.scale_log2));
+                const float f = ex2(reference_step<F16>(w[k], top, p.scale_log2));
                 sum = fmaf(f, s[k], sum);
                 a = fmaf(f, x[k], a);
                 b = fmaf(f, y[k], b);

@@ -1,5 +1,7 @@
-"""rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds, and rows
-whose every score is -infinity."""
+"""rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds, rows
+whose every score is -infinity, and the many small probabilities of a long text."""
+
+import math
 
 import pytest
 
@@ -180,3 +182,26 @@ def test_minus_infinities_in_split_keys(cuda, q, keys, heads, kv_heads, dim):
     status(torch)
     v = b.kv[keys - 1, kv_heads * dim:].view(kv_heads, 1, dim).expand(kv_heads, heads // kv_heads, dim).reshape(1, -1)
     assert torch.equal(got, v.expand(q, -1))
+
+
+@pytest.mark.parametrize("q,heads,kv_heads,dim", [(1, 1, 1, 32), (3, 2, 2, 64), (2000, 1, 1, 64), (2000, 2, 1, 128), (1500, 1, 1, 256)])
+def test_many_small_probabilities_in_fp16(cuda, q, heads, kv_heads, dim):
+    """One key with nearly all the weight over a text of 2^17: the others' 2^-27 each are below the steps of fp16, but
+    a thousandth together.  V is 0 at the first and 1 at the others, so that the result is that thousandth, off by its
+    rounding (2^-11), the probabilities' (2^-11, or 2^-25 of the largest value of P there is, 2^7 and more), the
+    exponentials' (2^-16) and the sums' additions ((keys + 16) 2^-23 of it)."""
+    torch = cuda
+    n = 1 << 17
+    b = Batch(torch, [q], [n], heads, kv_heads, dim, "f16", 99)
+    b.q.zero_()
+    b.kv.zero_()
+    b.q[:q, :heads * dim:dim] = 1.0
+    b.kv[0, :kv_heads * dim:dim] = 18.75
+    b.kv[1:, kv_heads * dim:] = 1.0
+    b.scale = 1.0
+    b.run()
+    status(torch)
+    w = (n - 1) * math.exp(-18.75)
+    want = w / (1 + w)
+    got = b.out[:q, :heads * dim].double()
+    assert float((got - want).abs().max()) <= (2.0**-10 + 2.0**-16 + (n + 16) * 2.0**-23) * want + n * 2.0**-32
