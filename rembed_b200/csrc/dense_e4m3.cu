@@ -518,6 +518,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
         uint8_t* box = boxes + ew * S::BOXES;
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+        // TMA writes whole 16 bytes, zeros behind column N
+        const bool whole = p.N % (O == Elem::kF32 ? 4 : 8) == 0;
         int acc = 0, slot = 0, stores = 0;
         uint32_t acc_phase = 0, slot_phase = 0;
         bool ok = true;
@@ -591,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                     for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
                     if (row < p.M && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
                 }
-                if (tma_out) {
+                if (tma_out && (c0 + 32 <= p.N || whole)) {
                     // the store that last read this box has left it
                     uint8_t* b = O == Elem::kF32 ? box : box + (stores & 1) * 2048;
                     if (lane == 0) {
@@ -621,8 +623,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                     }
                     ++stores;
                 } else {
-                    // rows of y that TMA cannot address: through shared memory, so
-                    // that a warp writes 32 neighbours of one row
+                    // rows of y that TMA cannot address, or the end of them: through
+                    // shared memory, so that a warp writes 32 neighbours of one row
+                    if (tma_out && lane == 0) bulk_wait_read<0>();
+                    __syncwarp();
                     float* f = reinterpret_cast<float*>(box);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) f[lane * 32 + (i ^ lane)] = v[i];

@@ -1,11 +1,11 @@
-"""The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, and
-values at and beside ties."""
+"""The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, values
+at and beside ties, and rows of y that end within 16 bytes."""
 
 import numpy as np
 import pytest
 
 import e4m3_reference as ref
-from test_gpu_e4m3 import DT, call, quantize, status, tdt
+from test_gpu_e4m3 import DT, call, check, dense, operands, quantize, status, tdt
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,14 @@ def test_the_same_values_give_the_same_bytes(cuda, tiles, dtype):
     q, s = quantize(torch, x, tiles)
     q32, s32 = quantize(torch, x.float(), tiles)
     assert np.array_equal(s, s32) and np.array_equal(q, q32), (q != q32).sum()
+
+
+@pytest.mark.parametrize("N", [601, 604, 606, 607, 608, 31])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_columns_behind_the_last_stay(cuda, N, dtype):
+    """Rows of y that start on 16-byte boundaries and end between them: what lies behind column N is left alone."""
+    torch = cuda
+    host, ops = operands(torch, 700, N, 512, N)
+    y = dense(torch, ops, 700, N, 512, None, dtype, ldy=N + 16 - N % 8)
+    status(torch)
+    check(torch, y, host, None, dtype, 700, N, 512, N + 16 - N % 8, 0)
