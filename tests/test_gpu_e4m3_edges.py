@@ -1,5 +1,6 @@
 """The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, values
-at and beside ties, and rows of y that end within 16 bytes."""
+at and beside ties, rows of y that end within 16 bytes, products of several tiles for each pair of CTAs, splits of K of
+every size, and infinite scales."""
 
 import numpy as np
 import pytest
@@ -100,3 +101,45 @@ def test_columns_behind_the_last_stay(cuda, N, dtype):
     y = dense(torch, ops, 700, N, 512, None, dtype, ldy=N + 16 - N % 8)
     status(torch)
     check(torch, y, host, None, dtype, 700, N, 512, N + 16 - N % 8, 0)
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 4500, 100), (4100, 4500, 1100), (4100, 1100, 300), (20000, 300, 260), (5000, 2100, 1100)])
+def test_pairs_walk_several_tiles(cuda, M, N, K):
+    """Two to five tiles, 256 wide and 128 wide, for each of the 74 pairs of CTAs there are at most: rings, accumulators,
+    scales and output boxes carried from one to the next, with one block of K, three and nine.  Outputs by TMA (a
+    stride of 16 bytes' multiple) and not."""
+    torch = cuda
+    assert -(-M // 256) * -(-N // 256) > 74 or -(-M // 256) * -(-N // 128) > 2 * 74
+    host, ops = operands(torch, M, N, K, M + K)
+    bias = torch.randn((N,), device="cuda")
+    for dtype in ("f32", "bf16", "f16"):
+        for pad in (3, 4):
+            y = dense(torch, ops, M, N, K, bias, dtype, ldy=N + pad)
+            status(torch)
+            check(torch, y, host, bias, dtype, M, N, K, N + pad, 0)
+
+
+@pytest.mark.parametrize("M,N,K", [(64, 19200, 1700), (50, 19199, 1700), (64, 12800, 3300), (60, 12700, 3300), (40, 6300, 3300)])
+def test_few_rows_and_many_columns(cuda, M, N, K):
+    """So many tiles of columns that K is not split, or over two CTAs, or four."""
+    torch = cuda
+    host, ops = operands(torch, M, N, K, M + N)
+    bias = torch.randn((N,), device="cuda")
+    for dtype in ("f32", "bf16"):
+        y = dense(torch, ops, M, N, K, bias, dtype)
+        status(torch)
+        check(torch, y, host, bias, dtype, M, N, K, N, 0)
+
+
+@pytest.mark.parametrize("M", [5, 40, 700])
+def test_dense_infinite_weight_scale(cuda, M):
+    """One block of 128 x 128 weights with an infinite scale: its columns are infinite or NaN, all others as without."""
+    torch = cuda
+    _, ops = operands(torch, M, 400, 384, 6)
+    clean = dense(torch, ops, M, 400, 384, None, "f32")
+    ops[3][1, 2] = float("inf")
+    dirty = dense(torch, ops, M, 400, 384, None, "f32")
+    status(torch)
+    a, b = (t[:M * 400].view(M, 400).cpu().numpy() for t in (clean, dirty))
+    assert not np.isfinite(b[:, 128:256]).any()
+    assert np.array_equal(np.delete(a, np.s_[128:256], 1), np.delete(b, np.s_[128:256], 1))
