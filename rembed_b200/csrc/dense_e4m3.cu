@@ -332,7 +332,12 @@ __device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
     return d;
 }
 
-template <int BN, Elem O>
+// RAGGED: the rows of y, written by TMA, end between 16 bytes.  TMA writes whole
+// ones, zeros behind the row, so that their last box goes out by plain stores (a
+// kernel of its own: as a test in the other it moved registers about in the loop
+// over K, 16384 x 4096 x 4096 276 against 267 us; y without TMA took 348 us where
+// N = 4100).
+template <int BN, Elem O, bool RAGGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
     dense_e4m3_wide_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                            const __grid_constant__ CUtensorMap tmY, DenseE4Params p, bool tma_out) {
@@ -518,8 +523,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
         uint8_t* box = boxes + ew * S::BOXES;
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-        // TMA writes whole 16 bytes, zeros behind column N
-        const bool whole = p.N % (O == Elem::kF32 ? 4 : 8) == 0;
         int acc = 0, slot = 0, stores = 0;
         uint32_t acc_phase = 0, slot_phase = 0;
         bool ok = true;
@@ -593,7 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                     for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
                     if (row < p.M && amax > 65504.0f) atomicOr(p.status, kStatusF16Overflow);
                 }
-                if (tma_out && (c0 + 32 <= p.N || whole)) {
+                if (tma_out && (!RAGGED || c0 + 32 <= p.N)) {
                     // the store that last read this box has left it
                     uint8_t* b = O == Elem::kF32 ? box : box + (stores & 1) * 2048;
                     if (lane == 0) {
@@ -623,10 +626,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(384, 1)
                     }
                     ++stores;
                 } else {
-                    // rows of y that TMA cannot address, or the end of them: through
-                    // shared memory, so that a warp writes 32 neighbours of one row
-                    if (tma_out && lane == 0) bulk_wait_read<0>();
-                    __syncwarp();
+                    // rows of y that TMA cannot address: through shared memory, so
+                    // that a warp writes 32 neighbours of one row
+                    if (RAGGED) {
+                        if (lane == 0) bulk_wait_read<0>();
+                        __syncwarp();
+                    }
                     float* f = reinterpret_cast<float*>(box);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) f[lane * 32 + (i ^ lane)] = v[i];
@@ -696,19 +701,19 @@ cudaError_t launch_thin(const DenseE4Params& p, int split, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, tw, tx, p, split);
 }
 
-template <int BN, Elem O>
-cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
+template <int BN, Elem O, bool RAGGED>
+cudaError_t launch_wide_as(const DenseE4Params& p, const CUtensorMap* out, int num_sms, cudaStream_t st) {
     using S = WideShape<BN>;
     static unsigned configured = 0;
-    auto kern = dense_e4m3_wide_kernel<BN, O>;
+    auto kern = dense_e4m3_wide_kernel<BN, O, RAGGED>;
     cudaError_t e = allow_smem(kern, S::SMEM, configured);
     if (e != cudaSuccess) return e;
-    CUtensorMap tx, tw, ty;
+    CUtensorMap tx, tw;
     if (!make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, 128) ||
         !make_kmajor_tmap(&tw, p.wq, 1, p.N, p.K, p.ldw, S::HALF))
         return cudaErrorInvalidValue;
-    const bool tma_out = make_epilogue_tmap(&ty, p.y, O == Elem::kF32, O == Elem::kF16, p.M, p.N, p.ldy);
-    if (!tma_out) ty = tx;  // not read
+    const bool tma_out = out != nullptr;
+    const CUtensorMap ty = out ? *out : tx;  // not read without
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
     // one pair per tile slot: as many as can be resident at once
     static int resident[32] = {};
@@ -735,6 +740,15 @@ cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
     }
     const dim3 grid(2 * static_cast<unsigned>(tiles < pairs ? tiles : pairs));
     return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tx, tw, ty, p, tma_out);
+}
+
+template <int BN, Elem O>
+cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
+    CUtensorMap ty;
+    if (!make_epilogue_tmap(&ty, p.y, O == Elem::kF32, O == Elem::kF16, p.M, p.N, p.ldy))
+        return launch_wide_as<BN, O, false>(p, nullptr, num_sms, st);
+    if (p.N % (O == Elem::kF32 ? 4 : 8) == 0) return launch_wide_as<BN, O, false>(p, &ty, num_sms, st);
+    return launch_wide_as<BN, O, true>(p, &ty, num_sms, st);
 }
 
 // Up to 32 rows the weights' bytes count, and the thin kernel spreads them over
