@@ -59,24 +59,24 @@ bool make_w8_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t co
     return r == CUDA_SUCCESS;
 }
 
-// Output / residual maps: boxes of 32 rows x box_cols columns, rows of 128 bytes (fp32, 128-byte
+// Output / residual maps: 32 x 32 boxes, rows of 128 bytes (fp32, 128-byte
 // swizzle) or 64 bytes (16-bit, 64-byte swizzle), matching the kernel's
 // staging-box layout (swz in gemm_impl.cuh).
 bool make_epilogue_tmap(CUtensorMap* map, const void* base, bool f32, bool f16, uint64_t rows, uint64_t cols,
-                        uint64_t ld, uint32_t box_cols) {
+                        uint64_t ld) {
     EncodeTiledFn fn = encode_fn();
     if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) != 0) return false;
     const uint64_t eb = f32 ? 4 : 2;
     if ((ld * eb) % 16 != 0) return false;
     cuuint64_t dims[2] = {cols, rows};
     cuuint64_t strides[1] = {ld * eb};
-    cuuint32_t box[2] = {box_cols, 32};
+    cuuint32_t box[2] = {32, 32};
     cuuint32_t estr[2] = {1, 1};
     const CUtensorMapDataType dt = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : (f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
     CUresult r = fn(map, dt, 2,
                     const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    box_cols * eb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }

@@ -109,12 +109,12 @@ struct GemmMaps {
 // elem_bytes: 4 (fp32), 2 (bf16 / fp16) or 1 (int8).  Returns false on failure.
 bool make_kmajor_tmap(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
                       uint64_t row_stride_elems, uint32_t box_rows);
-// Tensor map over an fp32 (f32), fp16 (f16) or bf16 matrix for boxes of 32 rows
-// x box_cols columns, staged as rows of 128 bytes (128-byte swizzle) or 64
-// bytes (64-byte swizzle).  Returns false unless base and row stride are
-// 16-byte aligned.
+// Tensor map over an fp32 (f32), fp16 (f16) or bf16 matrix for boxes of 32 x 32,
+// staged as rows of 128 bytes (128-byte swizzle) or 64 bytes (64-byte swizzle).
+// Returns false unless base and row stride are 16-byte aligned.  A store writes
+// whole 16 bytes: zeros behind rows of cols that end between them.
 bool make_epilogue_tmap(CUtensorMap* map, const void* base, bool f32, bool f16, uint64_t rows, uint64_t cols,
-                        uint64_t ld, uint32_t box_cols = 32);
+                        uint64_t ld);
 // Tensor map over an int8 weight [rows x cols] for GemmKind::kW8: boxes of
 // 64 bytes of K x box_rows, unswizzled.
 bool make_w8_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
