@@ -87,25 +87,6 @@ struct Const {
 // registers of the two-tile kernel: 128 * 72 + 256 * 216 = 384 * 168
 constexpr int kControlRegs = 72, kSoftmaxRegs = 216;
 
-// Pairs of floats in one 64-bit register: half the instructions.
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split_pair(uint64_t r, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 // 2^x of a pair on the FMA pipe: n = round(x) by the magic constant 1.5 * 2^23,
 // 2^f on [-1/2, 1/2] by a quartic fitted here for least relative error (2.7e-6
 // in fp32), n added to the exponent.  Clamped at 2^-125, which is nothing beside

@@ -31,7 +31,9 @@ constexpr int kRows = 16;
 template <int D>
 struct RowsShape {
     static constexpr int KEYS = D <= 64 ? 32 : 16;  // keys of a chunk
-    static constexpr int STAGES = D == 32 ? 4 : 2;  // of chunks; three CTAs an SM (head dim 256: one)
+    // of chunks: room for three CTAs an SM (head dim 256: one); keys are split while
+    // the parts fit two an SM
+    static constexpr int STAGES = D == 32 ? 4 : 2;
     static constexpr int CHUNK = KEYS * D * 2;  // bytes of a chunk of K, and of V
     static constexpr int RING = STAGES * 2 * CHUNK;
     // at the end a warp's 16 x D fp32 outputs take its ring's place

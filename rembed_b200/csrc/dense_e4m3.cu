@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "act16.cuh"
+#include "clusters.cuh"
 #include "e4m3.cuh"
 #include "gemm.cuh"
 #include "pdl.cuh"
@@ -313,24 +314,10 @@ struct WideShape {
     static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + WARPS * BOXES + SR * 1024 + 1024 + 512;
     static constexpr int THREADS = 128 + 32 * WARPS;
     // 128 * 24 + 256 * 240 = 384 * 168; with 232 for the sums their pairs are
-    // moved about (16384 x 4096 x 4096: 255 against 243 us)
+    // moved about (16384 x 4096 x 4096: 255 against 243 us); 20 to 36 bytes are spilled
     static constexpr int CONTROL_REGS = 24, SUM_REGS = 240;
     static_assert(SMEM <= 232448, "shared memory");
 };
-
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split_pair(uint64_t r, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 
 // RAGGED: the rows of y, written by TMA, end between 16 bytes.  TMA writes whole
 // ones, zeros behind the row, so that their last box goes out by plain stores (a
@@ -661,9 +648,11 @@ cudaError_t allow_smem(K kern, int bytes, unsigned& configured) {
 }
 
 // K is split over up to eight CTAs (of at least four rows each in the join)
-// while they all run at once: two an SM, of which clusters of four and eight
-// leave a tenth empty, as they do not cross GPCs (256 of them ran at once; of 288
-// and 296 some waited: 100 x 4736 x 16384 47 us over four, 39 over two).
+// while they all run at once.  That is two an SM, which the occupancy query does
+// not know (it counts one CTA an SM for kernels that allocate tensor memory), so
+// that the bound is a measured one: clusters of four and eight leave a tenth of
+// the places empty, as they do not cross GPCs (of 256 CTAs all ran at once, of
+// 288 and 296 some waited: 100 x 4736 x 16384 47 us over four, 39 over two).
 int thin_split(const DenseE4Params& p, int nt, int num_sms) {
     const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + nt - 1) / nt);
     const int kblocks = (p.K + kE4Block - 1) / kE4Block;
@@ -702,11 +691,12 @@ cudaError_t launch_thin(const DenseE4Params& p, int split, cudaStream_t st) {
 }
 
 template <int BN, Elem O, bool RAGGED>
-cudaError_t launch_wide_as(const DenseE4Params& p, const CUtensorMap* out, int num_sms, cudaStream_t st) {
+cudaError_t launch_wide_as(const DenseE4Params& p, const CUtensorMap* out, cudaStream_t st) {
     using S = WideShape<BN>;
-    static unsigned configured = 0;
+    static ClusterCounts known = {};
     auto kern = dense_e4m3_wide_kernel<BN, O, RAGGED>;
-    cudaError_t e = allow_smem(kern, S::SMEM, configured);
+    int pairs = 0;  // one per tile slot: as many as can be resident at once
+    cudaError_t e = clusters_at_once(kern, S::THREADS, S::SMEM, 2, known, pairs);
     if (e != cudaSuccess) return e;
     CUtensorMap tx, tw;
     if (!make_kmajor_tmap(&tx, p.xq, 1, p.M, p.K, p.ldx, 128) ||
@@ -715,40 +705,17 @@ cudaError_t launch_wide_as(const DenseE4Params& p, const CUtensorMap* out, int n
     const bool tma_out = out != nullptr;
     const CUtensorMap ty = out ? *out : tx;  // not read without
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
-    // one pair per tile slot: as many as can be resident at once
-    static int resident[32] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int pairs = dev < 32 ? __atomic_load_n(&resident[dev], __ATOMIC_ACQUIRE) : 0;
-    if (pairs == 0) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(2 * (num_sms / 2));
-        cfg.blockDim = dim3(S::THREADS);
-        cfg.dynamicSmemBytes = S::SMEM;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = 2;
-        attr.val.clusterDim.y = 1;
-        attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs <= 0) {
-            cudaGetLastError();
-            pairs = num_sms / 2;
-        }
-        if (dev < 32) __atomic_store_n(&resident[dev], pairs, __ATOMIC_RELEASE);
-    }
     const dim3 grid(2 * static_cast<unsigned>(tiles < pairs ? tiles : pairs));
     return launch_pdl(kern, grid, dim3(S::THREADS), S::SMEM, st, tx, tw, ty, p, tma_out);
 }
 
 template <int BN, Elem O>
-cudaError_t launch_wide(const DenseE4Params& p, int num_sms, cudaStream_t st) {
+cudaError_t launch_wide(const DenseE4Params& p, cudaStream_t st) {
     CUtensorMap ty;
     if (!make_epilogue_tmap(&ty, p.y, O == Elem::kF32, O == Elem::kF16, p.M, p.N, p.ldy))
-        return launch_wide_as<BN, O, false>(p, nullptr, num_sms, st);
-    if (p.N % (O == Elem::kF32 ? 4 : 8) == 0) return launch_wide_as<BN, O, false>(p, &ty, num_sms, st);
-    return launch_wide_as<BN, O, true>(p, &ty, num_sms, st);
+        return launch_wide_as<BN, O, false>(p, nullptr, st);
+    if (p.N % (O == Elem::kF32 ? 4 : 8) == 0) return launch_wide_as<BN, O, false>(p, &ty, st);
+    return launch_wide_as<BN, O, true>(p, &ty, st);
 }
 
 // Up to 32 rows the weights' bytes count, and the thin kernel spreads them over
@@ -777,8 +744,8 @@ cudaError_t launch_out(const DenseE4Params& p, int num_sms, cudaStream_t st) {
         const float thin = 3.0f + block * static_cast<float>((kblocks + split - 1) / split);
         if (thin <= std::min(wide256, wide128) * static_cast<float>(kblocks)) return launch_thin<64, O>(p, split, st);
     }
-    if (wide128 < wide256) return launch_wide<128, O>(p, num_sms, st);
-    return launch_wide<256, O>(p, num_sms, st);
+    if (wide128 < wide256) return launch_wide<128, O>(p, st);
+    return launch_wide<256, O>(p, st);
 }
 
 }  // namespace

@@ -102,10 +102,10 @@ rg::Elem elem_of(int dtype) {
     return dtype == RG_DTYPE_F32 ? rg::Elem::kF32 : (dtype == RG_DTYPE_F16 ? rg::Elem::kF16 : rg::Elem::kBF16);
 }
 
-// The two e4m3 quantisers' common checks; fills p.
 // Row and column numbers of the last, partly filled tile stay within 32 bits.
 constexpr int kMaxExtent = 0x7fffff00;
 
+// The two e4m3 quantisers' common checks; fills p.
 int quant_e4m3_args(const char* fn, const void* x, int dtype, int ldx, int rows, int K, uint8_t* q, int ldq,
                     float* scale, rg::QuantE4Params* p, char** err) {
     if (!x || !q || !scale) return set_err(err, "%s: null buffer", fn);
