@@ -1,8 +1,11 @@
 """rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds, rows
-whose every score is -infinity, and the many small probabilities of a long text."""
+whose every score is -infinity, and the many small probabilities of a long text.  Then the operators behind an
+encoder's forward pass."""
 
+import ctypes
 import math
 
+import numpy as np
 import pytest
 
 from test_gpu_cross_attention import HEADS, Batch, status
@@ -205,3 +208,47 @@ def test_many_small_probabilities_in_fp16(cuda, q, heads, kv_heads, dim):
     want = w / (1 + w)
     got = b.out[:q, :heads * dim].double()
     assert float((got - want).abs().max()) <= (2.0**-10 + 2.0**-16 + (n + 16) * 2.0**-23) * want + n * 2.0**-32
+
+
+def test_behind_an_encoder(cuda):
+    """An encoder's forward pass leaves its token states on the device; they are quantised, projected to K and V, and
+    attended to by prompts and then by single tokens, all on one stream without a synchronisation.  K and V are held to
+    the exact projection of the states (within the operands' 8-bit rounding), the attention to its inputs."""
+    from rembed_b200 import synth
+    from rembed_b200.embedder import Embedder, library
+
+    torch = cuda
+    lens, heads, dim = [40, 7, 131], 4, 64
+    cfg = synth.preset("minilm-l6")
+    enc = Embedder(cfg, synth.make_weights(cfg, seed=0))
+    H, T, N = cfg.hidden_size, sum(lens), 2 * heads * dim
+    cu = np.cumsum([0] + lens).astype(np.int32)
+    rng = np.random.default_rng(3)
+    ids = rng.integers(1000, 30000, T)
+    d_ids, d_cu = torch.from_numpy(ids).cuda(), torch.from_numpy(cu).cuda()
+    w = torch.randn((N, H), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)) * 0.03
+    states = torch.empty((T, H), device="cuda")
+    xq, wq = (torch.empty((r, H), device="cuda", dtype=torch.uint8) for r in (T, N))
+    xs, ws = torch.empty((H // 128, T), device="cuda"), torch.empty((N // 128, H // 128), device="cuda")
+    prompt = Batch(torch, [60, 1, 9], lens, heads, heads, dim, "bf16", 4)
+    step = Batch(torch, [1, 1, 1], lens, heads, heads, dim, "bf16", 5)
+    step.kv = prompt.kv
+    torch.cuda.synchronize()
+    lib, err, at = library(), ctypes.c_char_p(), torch.cuda.Stream().cuda_stream
+    enc.forward_device(d_ids.data_ptr(), d_cu.data_ptr(), cu, states.data_ptr(), stream=at, tokens=True)
+    assert lib.rg_quantize_tiles_e4m3(w.data_ptr(), 0, H, N, H, wq.data_ptr(), H, ws.data_ptr(), at, ctypes.byref(err)) == 0
+    assert lib.rg_quantize_rows_e4m3(states.data_ptr(), 0, H, T, H, xq.data_ptr(), H, xs.data_ptr(), T, at, ctypes.byref(err)) == 0
+    assert lib.rg_dense_e4m3(xq.data_ptr(), H, xs.data_ptr(), T, wq.data_ptr(), H, ws.data_ptr(), None, prompt.kv.data_ptr(), N, 2,
+                             T, N, H, at, ctypes.byref(err)) == 0
+    prompt.run(stream=at)
+    step.run(stream=at)
+    torch.cuda.synchronize()
+    enc.sync()
+    status(torch)
+    vectors = enc.embed_tokens([ids[a:b] for a, b in zip(cu[:-1], cu[1:])])
+    assert np.array_equal(states.cpu().numpy(), np.concatenate([v.vectors for v in vectors]))
+    exact = states.double() @ w.double().t()
+    # independent errors of two factors, each of rms below 2^-3 / sqrt(12) of itself, and the result's rounding
+    assert float((prompt.kv.double() - exact).norm() / exact.norm()) <= math.sqrt(2) * 2.0**-3 / math.sqrt(12) + 2.0**-8
+    prompt.check()
+    step.check()
