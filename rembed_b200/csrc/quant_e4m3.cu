@@ -38,10 +38,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return y;
 }
 
-// x (r + d) rounded so that its rounding to e4m3 is that of the exact product.
+// x (r + d) rounded so that its rounding to e4m3 is that of the exact product; the
+// remainder is subtracted, so that a zero keeps its sign.
 __device__ __forceinline__ float scaled16(float x, float2 inv) {
     const float y = __fmul_rn(x, inv.x);
-    return __fadd_rn(y, __fmaf_rn(x, inv.y, __fmaf_rn(x, inv.x, -y)));
+    return __fsub_rn(y, __fmaf_rn(-x, inv.y, __fmaf_rn(-x, inv.x, y)));
 }
 
 // The e4m3 byte of x over a block of maximum a (448 2^-126 at least), given the

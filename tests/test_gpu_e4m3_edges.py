@@ -1,6 +1,6 @@
 """The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, values
 at and beside ties, rows of y that end within 16 bytes, products of several tiles for each pair of CTAs, splits of K of
-every size, and infinite scales."""
+every size, infinite scales, and special values of 16 bits."""
 
 import numpy as np
 import pytest
@@ -90,6 +90,28 @@ def test_the_same_values_give_the_same_bytes(cuda, tiles, dtype):
     q, s = quantize(torch, x, tiles)
     q32, s32 = quantize(torch, x.float(), tiles)
     assert np.array_equal(s, s32) and np.array_equal(q, q32), (q != q32).sum()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_special_values_of_16_bits(cuda, tiles, dtype, pad):
+    """Zeros of both signs, subnormals, the largest values, NaN and infinities in 16 bits: each block for itself."""
+    torch = cuda
+    big, tiny = (65504.0, 2.0**-24) if dtype == "f16" else (3.38e38, 2.0**-133)
+    x = torch.zeros((256, 512 + pad))
+    x[:, 1] = -0.0
+    x[0, 128:256] = tiny
+    x[1, 256:384] = torch.linspace(-big, big, 128)
+    x[130, 5], x[130, 6] = float("nan"), 2.0
+    x[131, 300], x[131, 301] = -float("inf"), 2.0
+    x[132, 400], x[132, 401] = float("inf"), float("nan")
+    x = x.to(tdt(torch, dtype)).cuda()[:, :512]
+    q, s = quantize(torch, x, tiles)
+    want_q, want_s = ref.quantize(x.float().cpu().numpy(), 128 if tiles else 1)
+    assert np.array_equal(s if tiles else s.T, want_s, equal_nan=True)
+    nan = np.isnan(ref.decode(want_q))
+    assert np.array_equal(np.isnan(ref.decode(q)), nan) and np.array_equal(q[~nan], want_q[~nan])
 
 
 @pytest.mark.parametrize("N", [601, 604, 606, 607, 608, 31])
