@@ -1,6 +1,6 @@
 """rg_cross_attention at the ends of its range: scores far beyond what a probability's exponent holds, rows
-whose every score is -infinity, and the many small probabilities of a long text.  Then the operators behind an
-encoder's forward pass."""
+whose every score is -infinity, the many small probabilities of a long text, and buffers of gigabytes.  Then the
+operators behind an encoder's forward pass."""
 
 import ctypes
 import math
@@ -208,6 +208,29 @@ def test_many_small_probabilities_in_fp16(cuda, q, heads, kv_heads, dim):
     want = w / (1 + w)
     got = b.out[:q, :heads * dim].double()
     assert float((got - want).abs().max()) <= (2.0**-10 + 2.0**-16 + (n + 16) * 2.0**-23) * want + n * 2.0**-32
+
+
+@pytest.mark.parametrize("q", [1, 3, 200])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 128), (16, 2, 256)])
+def test_texts_and_rows_beyond_2_32_bytes(cuda, q, heads, kv_heads, dim):
+    """A text at the end of a cache of 8 GiB, queries and outputs at the end of buffers of 8 GiB, with anything before."""
+    torch = cuda
+    b = Batch(torch, [q, q], [700, 41], heads, kv_heads, dim, "bf16", 95)
+    first_q, first_k = 2**20, 2**22
+    big = lambda rows, like: torch.empty((rows + like.shape[0], like.shape[1]), device="cuda", dtype=like.dtype)  # noqa: E731
+    far = Batch(torch, [q, q], [700, 41], heads, kv_heads, dim, "bf16", 95)
+    far.q, far.kv, far.out = big(first_q, b.q), big(first_k, b.kv), big(first_q, b.out)
+    far.q[first_q:], far.kv[first_k:], far.out[first_q:] = b.q, b.kv, -7.0
+    assert far.q.numel() > 2**32 and far.kv.numel() >= 2**32 and far.out.numel() > 2**32
+    far.tables[0] += first_q
+    far.tables[1] += first_k
+    far.Tq += first_q
+    far.Tk += first_k
+    b.run()
+    far.run()
+    status(torch)
+    b.check()
+    assert torch.equal(far.out[first_q:], b.out)
 
 
 def test_behind_an_encoder(cuda):

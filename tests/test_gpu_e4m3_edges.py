@@ -1,6 +1,6 @@
 """The e4m3 path where it can go wrong beyond its ordinary shapes: rows of more than 2^31 bytes, values
 at and beside ties, rows of y that end within 16 bytes, products of several tiles for each pair of CTAs, splits of K of
-every size, infinite scales, and special values of 16 bits."""
+every size, infinite scales, special values of 16 bits, and outputs whose rows lie gigabytes apart."""
 
 import numpy as np
 import pytest
@@ -93,6 +93,21 @@ def test_the_same_values_give_the_same_bytes(cuda, tiles, dtype):
 
 
 @pytest.mark.parametrize("tiles", [False, True])
+def test_ties_over_the_smallest_scale(cuda, tiles):
+    """Blocks whose maximum over 448 would be no normal number: x / 2^-126, ties and their neighbours among them."""
+    torch = cuda
+    rng = np.random.default_rng(7)
+    t = midpoints()
+    x = rng.choice(t[t <= 300], (512, 128)) * 2.0**-126
+    x = (x + rng.integers(-2, 3, x.shape) * 2.0**-149 * (rng.random(x.shape) < 0.5)).astype(np.float32)
+    x *= rng.choice([-1, 1], x.shape).astype(np.float32)
+    q, s = quantize(torch, torch.from_numpy(x).cuda(), tiles)
+    want_q, want_s = ref.quantize(x, 128 if tiles else 1)
+    assert (want_s == np.float32(2.0**-126)).all() and np.array_equal(s if tiles else s.T, want_s)
+    assert np.array_equal(q, want_q)
+
+
+@pytest.mark.parametrize("tiles", [False, True])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("pad", [0, 1])
 def test_special_values_of_16_bits(cuda, tiles, dtype, pad):
@@ -165,3 +180,17 @@ def test_dense_infinite_weight_scale(cuda, M):
     a, b = (t[:M * 400].view(M, 400).cpu().numpy() for t in (clean, dirty))
     assert not np.isfinite(b[:, 128:256]).any()
     assert np.array_equal(np.delete(a, np.s_[128:256], 1), np.delete(b, np.s_[128:256], 1))
+
+
+@pytest.mark.parametrize("M,K,ldy", [(5, 300, 2**29), (40, 3000, 2**27), (300, 300, 2**24), (300, 300, 2**24 + 1)])
+def test_rows_of_y_far_apart(cuda, M, K, ldy):
+    """Rows whose offsets pass 2^31 elements and 2^32 bytes, from every kernel and by both ways of writing y."""
+    torch = cuda
+    N = 136
+    host, ops = operands(torch, M, N, K, M)
+    y = torch.empty((M * ldy,), device="cuda", dtype=torch.bfloat16)
+    rows = y.view(M, ldy)[:, :N + 8]
+    rows.fill_(-77.0)
+    dense(torch, ops, M, N, K, None, "bf16", ldy=ldy, y=y)
+    status(torch)
+    check(torch, torch.cat([rows.reshape(-1), rows.new_full((5,), -77.0)]), host, None, "bf16", M, N, K, N + 8, 0)
