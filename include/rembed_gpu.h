@@ -278,8 +278,8 @@ int rg_dense_s8(const int8_t *xq, const float *row_scale, const int8_t *wq, cons
  * rg_dense_e4m3 reads q with ldq a multiple of 16 from a 16-byte aligned
  * base.
  *
- * rg_quantize_tiles_e4m3: the same for the tiles of a weight w [N x K]:
- * scale[(n / 128) * ceil(K / 128) + b], contiguous. */
+ * rg_quantize_tiles_e4m3: the same for the tiles of a weight w [N x K], N up
+ * to 8 388 480: scale[(n / 128) * ceil(K / 128) + b], contiguous. */
 int rg_quantize_rows_e4m3(const void *x, int dtype, int ldx, int M, int K, uint8_t *q, int ldq, float *scale,
                           int ld_scale, void *stream, char **err);
 int rg_quantize_tiles_e4m3(const void *w, int dtype, int ldw, int N, int K, uint8_t *q, int ldq, float *scale,
@@ -288,7 +288,8 @@ int rg_quantize_tiles_e4m3(const void *w, int dtype, int ldw, int N, int K, uint
 /* rg_dense_e4m3: the projection over such operands,
  * y[m][n] = sum_b x_scale[b * ld_xs + m] * w_scale[n / 128][b] *
  *           sum_{k in block b} xq[m][k] * wq[n][k]   (+ bias[n]),
- * every sum in fp32.  xq [M x K] and wq [N x K] e4m3 with row strides ldx,
+ * every sum in fp32, after the two scales' product, which has to be within
+ * its range.  xq [M x K] and wq [N x K] e4m3 with row strides ldx,
  * ldw (multiples of 16, 16-byte aligned bases; columns from K on are not
  * read), scales as the quantisers write them, bias fp32 or NULL, y [M x N]
  * with row stride ldy in `dtype` (RG_DTYPE_F32, F16 or BF16; columns from N
@@ -311,7 +312,9 @@ int rg_dense_e4m3(const uint8_t *xq, int ldx, const float *x_scale, int ld_xs, c
  * output is zeros.  Rows of out outside every sequence are left alone.  Scores
  * are fp32 sums of products; finite ones may be of any size, their product with
  * scale too (the largest then takes all the weight).  A row with a NaN or
- * +infinity among its scores, or with nothing but -infinities, is NaN.
+ * +infinity among its scores, or with nothing but -infinities, is NaN.  The
+ * softmax is held in fp32; probabilities are rounded to V's type where they
+ * meet V, as in rg_attention, and results once more.
  *
  * Heads as in rg_attention: query head h at columns h * head_dim, key/value
  * head h / (heads / kv_heads); head dims 32, 64, 128, 256; dtype
